@@ -28,7 +28,7 @@ extern "C" {
 
 #define Y3_VERSION 103
 
-enum { Y3_F32 = 0, Y3_BF16 = 1 };
+enum { Y3_F32 = 0, Y3_BF16 = 1, Y3_I8 = 2 };      /* Y3_I8: the 8-bit products only */
 
 enum {
     Y3_OK = 0,
@@ -281,6 +281,70 @@ int y3_pad_input(int dtype, const float *in, void *out, int64_t pixels, int cin,
 /* fp32 -> bf16 round-to-nearest-even on device (weight/activation staging). */
 int y3_cast_f32_to_bf16(const float *in, void *out, int64_t n, void *stream);
 int y3_cast_bf16_to_f32(const void *in, float *out, int64_t n, void *stream);
+
+/* ---- products in 8-bit integers --------------------------------------------------------
+ * y[m][n] = act(s[m] * t[n] * sum_k q[m][k] * w[n][k] + bias[n]): a 1x1 convolution (build_model.py:113-179) over
+ * rows = pixels, or any linear layer over rows = tokens, with one scale per row and one per output channel.
+ * A row x is held as q = round_half_even(x * (127 / a)), s = a / 127, a = max(max_k |x_k|, 127 * 2^-126); a row with a
+ * NaN or an infinity gets s = NaN and q = 0, so that every product of it is NaN.  The sum is exact (32-bit integers;
+ * k <= 131071), hence the result does not depend on how the work is split.  act: identity, or leaky-ReLU (alpha = 0.1)
+ * with Y3_CONV_LEAKY.  No padding channel of `out` is written. */
+typedef struct y3_linear_i8_desc {
+    int32_t dtype;        /* type of x: Y3_F32 / Y3_BF16 (rows are quantised on the way), Y3_I8 (with x_scale)      */
+    int32_t out_dtype;    /* Y3_F32 or Y3_BF16                                                                     */
+    int32_t k, n;         /* inputs and outputs of a row                                                           */
+    int64_t rows;
+    int64_t x_ld, out_ld; /* elements between rows (>= k, >= n)                                                     */
+    int32_t k_pad, n_pad; /* packed weights, see y3_linear_i8_layout                                                */
+    int32_t flags;        /* Y3_CONV_LEAKY or 0                                                                    */
+    int32_t reserved;
+} y3_linear_i8_desc;
+
+/* x [rows][x_ld] (Y3_F32, Y3_BF16) -> q: 8-bit rows q_ld bytes apart, zero filled from k to the next multiple of 16, and
+ * scale[rows].  q is 16-byte aligned, q_ld a multiple of 16.  Y3_I8 copies rows to that pitch (scale may be NULL). */
+int y3_quantize_rows_i8(int dtype, const void *x, int64_t rows, int k, int64_t x_ld, void *q, int64_t q_ld, float *scale,
+                        void *stream);
+/* Host only: fills k_pad and n_pad from k and n.  The packed weights take k_pad * n_pad bytes. */
+int y3_linear_i8_layout(y3_linear_i8_desc *desc);
+/* Weights w [n][w_ld] (row n = output channel n) -> packed (16-byte aligned).  Y3_F32 / Y3_BF16: quantised by the rule
+ * above, scale[n] written.  Y3_I8: laid out only, the caller has the scales. */
+int y3_linear_i8_pack(const y3_linear_i8_desc *desc, int w_dtype, const void *w, int64_t w_ld, void *packed, float *scale,
+                      void *stream);
+/* Host only: what y3_linear_i8 wants as workspace for this descriptor (0 = none, NULL is fine). */
+int y3_linear_i8_workspace_bytes(const y3_linear_i8_desc *desc, int64_t *bytes);
+/* x_scale[rows] with Y3_I8 rows, NULL otherwise.  8-bit rows start on 16 bytes (x_ld a multiple of 16) and may be read up
+ * to k rounded up to 16.  bias[n] may be NULL.  workspace: 16-byte aligned, of this call alone until it has run.  x and
+ * out must not overlap. */
+int y3_linear_i8(const y3_linear_i8_desc *desc, const void *x, const float *x_scale, const void *w_packed,
+                 const float *w_scale, const float *bias, void *out, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- log probabilities of given classes --------------------------------------------------
+ * For each row of `classes` logits z: log p_c = z_c - log sum_j exp(z_j) of the class ids[row], the entropy
+ * -sum_j p_j log p_j (natural logarithms), and the `top` classes of the largest logits (ties: the lowest class first)
+ * with their log p.  For a head's class logits this is the class posterior of a box that holds one object: independent
+ * sigmoids p_c of which exactly one is on give P(c) proportional to p_c / (1 - p_c) = exp(z_c).
+ * Logits of -inf have probability 0.  A row of nothing but -inf: log p = -inf, entropy 0.  A row with a NaN or +inf: NaN.
+ * Sums are fp32 with the row's maximum taken out. */
+typedef struct y3_log_probs_desc {
+    int32_t dtype;        /* Y3_F32 or Y3_BF16                                                                     */
+    int32_t classes;      /* 1 .. 2^24                                                                             */
+    int64_t rows;
+    int64_t group_ld;     /* row r starts (r / group) * group_ld + (r % group) * row_ld elements behind `logits`:    */
+    int64_t row_ld;       /*   plain rows have group = 1, the boxes of a head's cells group = anchors               */
+    int32_t group;
+    int32_t top;          /* 0 .. 32, at most `classes`                                                            */
+    int32_t ids_64;       /* ids are int64 (otherwise int32)                                                       */
+    int32_t reserved;
+    int64_t extent;       /* elements that may be read from `logits` on                                            */
+} y3_log_probs_desc;
+
+/* row_offsets (nullable): element offset of each row instead of the strides above.  A negative offset skips the row: its
+ * outputs stay as they are.  A row that would end behind `extent` gets NaN and the class -1.
+ * ids (nullable with logp NULL): a negative id means no class, logp 0; an id >= classes gives NaN.
+ * logp[rows], entropy[rows] (nullable), top_ids[rows][top] and top_logp[rows][top] (NULL with top = 0). */
+int y3_log_probs_workspace_bytes(const y3_log_probs_desc *desc, int64_t *bytes);
+int y3_log_probs(const y3_log_probs_desc *desc, const void *logits, const int64_t *row_offsets, const void *ids, float *logp,
+                 float *entropy, int32_t *top_ids, float *top_logp, void *workspace, int64_t workspace_bytes, void *stream);
 
 int y3_version(void);
 const char *y3_last_error(void);

@@ -1,0 +1,120 @@
+"""The 8-bit product's and the class probabilities' refusals at the C-ABI: everything here is decided on the host, before
+any launch (no GPU)."""
+import ctypes
+
+import pytest
+
+from yolo_amd import _lib
+
+P = 1 << 12          # an aligned address nobody dereferences: every call below is refused first
+
+
+def linear(**kw):
+    d = _lib.LinearI8Desc()
+    d.dtype, d.out_dtype, d.k, d.n, d.rows, d.x_ld, d.out_ld = _lib.Y3_BF16, _lib.Y3_F32, 100, 50, 4, 100, 50
+    for k, v in kw.items():
+        setattr(d, k, v)
+    if 1 <= d.k <= 131071 and 1 <= d.n <= 1 << 24 and "k_pad" not in kw:
+        assert _lib.load().y3_linear_i8_layout(ctypes.byref(d)) == 0
+    return d
+
+
+def test_linear_layout(lib):
+    for k, n, kp, np_ in ((1, 1, 128, 16), (128, 16, 128, 16), (129, 17, 256, 32), (1024, 255, 1024, 256), (131071, 3, 131072, 16)):
+        d = linear(k=k, n=n, x_ld=k, out_ld=n)
+        assert (d.k_pad, d.n_pad) == (kp, np_)
+    for bad in (dict(k=0), dict(k=131072), dict(n=0), dict(n=(1 << 24) + 1)):
+        d = _lib.LinearI8Desc()
+        d.k, d.n = 8, 8
+        for k, v in bad.items():
+            setattr(d, k, v)
+        assert lib.y3_linear_i8_layout(ctypes.byref(d)) == -1
+    assert lib.y3_linear_i8_layout(None) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=3), dict(out_dtype=_lib.Y3_I8), dict(rows=-1), dict(rows=1 << 50), dict(x_ld=99), dict(out_ld=49),
+                                dict(flags=2), dict(k_pad=64, n_pad=64)])
+def test_linear_descriptor_refusals(lib, kw):
+    d = linear(**kw)
+    need = ctypes.c_int64(0)
+    assert lib.y3_linear_i8_workspace_bytes(ctypes.byref(d), ctypes.byref(need)) == -1
+    assert lib.y3_linear_i8(ctypes.byref(d), P, None, P, P, None, 1 << 30, P, 1 << 40, None) == -1
+    with pytest.raises(ValueError):
+        _lib.check(-1)
+
+
+def test_linear_pointer_refusals(lib):
+    d = linear()
+    call = lambda *a: lib.y3_linear_i8(ctypes.byref(d), *a, None)  # noqa: E731
+    big, out = 1 << 40, 1 << 30
+    assert call(None, None, P, P, None, out, P, big) == -1
+    assert call(P, None, None, P, None, out, P, big) == -1
+    assert call(P, None, P, None, None, out, P, big) == -1
+    assert call(P, None, P, P, None, None, P, big) == -1
+    assert call(P, P, P, P, None, out, P, big) == -1                # scales with float rows
+    assert call(P + 1, None, P, P, None, out, P, big) == -2
+    assert call(P, None, P + 8, P, None, out, P, big) == -2
+    assert call(P, None, P, P + 2, None, out, P, big) == -2
+    assert call(P, None, P, P, P + 1, out, P, big) == -2
+    assert call(P, None, P, P, None, out + 2, P, big) == -2
+    assert call(P, None, P, P, None, P + 8, P, big) == -1           # overlaps x
+    assert b"overlap" in lib.y3_last_error()
+    d = linear(dtype=_lib.Y3_I8)
+    assert call(P, None, P, P, None, out, None, 0) == -1             # 8-bit rows without scales
+    assert call(P, P, P, P, None, out, None, 0) == -2                # x_ld 100: rows do not start on 16 bytes
+    d = linear(dtype=_lib.Y3_I8, x_ld=112)
+    assert call(P + 4, P, P, P, None, out, None, 0) == -2
+    d = linear(rows=0)
+    assert call(None, None, None, None, None, None, None, 0) == 0
+
+
+def test_quantize_and_pack_refusals(lib):
+    q = lib.y3_quantize_rows_i8
+    assert q(5, P, 1, 8, 8, 1 << 20, 16, P, None) == -1
+    assert q(0, P, 1, 0, 8, 1 << 20, 16, P, None) == -1
+    assert q(0, P, -1, 8, 8, 1 << 20, 16, P, None) == -1
+    assert q(0, P, 1, 8, 7, 1 << 20, 16, P, None) == -1
+    assert q(0, P, 1, 8, 8, 1 << 20, 8, P, None) == -2
+    assert q(0, P, 1, 17, 17, 1 << 20, 16, P, None) == -2
+    assert q(0, P, 1, 8, 8, (1 << 20) + 8, 16, P, None) == -2
+    assert q(0, P, 1, 8, 8, P, 16, P, None) == -1
+    assert q(0, P, 1, 8, 8, 1 << 20, 16, None, None) == -1
+    assert q(0, None, 0, 8, 8, None, 16, None, None) == 0
+    d = linear()
+    pack = lambda *a: lib.y3_linear_i8_pack(ctypes.byref(d), *a, None)  # noqa: E731
+    assert pack(7, P, 100, P, P) == -1
+    assert pack(0, P, 99, P, P) == -1
+    assert pack(0, P, 100, P + 4, P) == -2
+    assert pack(0, P, 100, P, None) == -1
+    assert pack(0, None, 100, P, P) == -1
+
+
+def probs(**kw):
+    d = _lib.LogProbsDesc()
+    d.dtype, d.classes, d.rows, d.group, d.group_ld, d.row_ld, d.top, d.extent = _lib.Y3_F32, 80, 10, 1, 85, 0, 3, 9 * 85 + 80
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=2), dict(classes=0), dict(classes=(1 << 24) + 1), dict(rows=-1), dict(top=33), dict(top=-1),
+                                dict(classes=2), dict(extent=9 * 85 + 79), dict(group=0), dict(group_ld=-1), dict(row_ld=-1), dict(rows=11),
+                                dict(group=3, group_ld=256, row_ld=85, extent=3 * 256 + 79)])
+def test_log_probs_descriptor_refusals(lib, kw):
+    d = probs(**kw)
+    assert lib.y3_log_probs(ctypes.byref(d), P, None, P, P, P, P, P, P, 1 << 40, None) == -1
+
+
+def test_log_probs_pointer_refusals(lib):
+    d = probs()
+    call = lambda *a: lib.y3_log_probs(ctypes.byref(d), *a, P, 1 << 40, None)  # noqa: E731
+    assert call(None, None, P, P, P, P, P) == -1
+    assert call(P, None, None, P, P, P, P) == -1
+    assert call(P, None, P, None, P, P, P) == -1
+    assert call(P, None, P, P, P, None, P) == -1
+    assert call(P + 2, None, P, P, P, P, P) == -2
+    assert call(P, P + 4, P, P, P, P, P) == -2
+    assert call(P, None, P + 2, P, P, P, P) == -2
+    assert call(P, None, P, P, P + 1, P, P) == -2
+    d = probs(rows=0)
+    assert call(None, None, None, None, None, None, None) == 0

@@ -7,7 +7,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("YOLO3HIP_LIB") or os.path.join(_HERE, "libyolo3hip.so")     # override: A/B builds
 EXP_LIB_PATH = os.path.join(_HERE, "libyolo3hip_exp.so")       # -DY3_EXPERIMENTS flavour: tests and A/B tools only
 
-Y3_F32, Y3_BF16 = 0, 1
+Y3_F32, Y3_BF16, Y3_I8 = 0, 1, 2
 CONV_LEAKY, CONV_RESIDUAL, CONV_UPS2X, CONV_OUT_F32, CONV_IN_F32, CONV_REVERSE, CONV_POOL2 = 1, 2, 4, 8, 16, 32, 64
 
 c_int, c_i64, c_f32, c_vp = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -35,6 +35,18 @@ class DecodeDesc(ctypes.Structure):
                 ("head_ld", ctypes.c_int32 * 3), ("anchors", ((c_f32 * 2) * 3) * 3),
                 ("stride_x", c_f32 * 3), ("stride_y", c_f32 * 3), ("score_threshold", c_f32),
                 ("boxes_per_image", ctypes.c_int32)]
+
+
+class LinearI8Desc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "out_dtype", "k", "n")]
+                + [(n, ctypes.c_int64) for n in ("rows", "x_ld", "out_ld")]
+                + [(n, ctypes.c_int32) for n in ("k_pad", "n_pad", "flags", "reserved")])
+
+
+class LogProbsDesc(ctypes.Structure):
+    _fields_ = ([("dtype", ctypes.c_int32), ("classes", ctypes.c_int32)]
+                + [(n, ctypes.c_int64) for n in ("rows", "group_ld", "row_ld")]
+                + [(n, ctypes.c_int32) for n in ("group", "top", "ids_64", "reserved")] + [("extent", ctypes.c_int64)])
 
 
 # every symbol include/yolo3hip.h declares: name -> (restype, argtypes)
@@ -71,6 +83,13 @@ SIGNATURES = {
     "y3_pad_input": (c_int, [c_int, c_vp, c_vp, c_i64, c_int, c_vp]),
     "y3_cast_f32_to_bf16": (c_int, [c_vp, c_vp, c_i64, c_vp]),
     "y3_cast_bf16_to_f32": (c_int, [c_vp, c_vp, c_i64, c_vp]),
+    "y3_quantize_rows_i8": (c_int, [c_int, c_vp, c_i64, c_int, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "y3_linear_i8_layout": (c_int, [ctypes.POINTER(LinearI8Desc)]),
+    "y3_linear_i8_pack": (c_int, [ctypes.POINTER(LinearI8Desc), c_int, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "y3_linear_i8_workspace_bytes": (c_int, [ctypes.POINTER(LinearI8Desc), ctypes.POINTER(ctypes.c_int64)]),
+    "y3_linear_i8": (c_int, [ctypes.POINTER(LinearI8Desc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "y3_log_probs_workspace_bytes": (c_int, [ctypes.POINTER(LogProbsDesc), ctypes.POINTER(ctypes.c_int64)]),
+    "y3_log_probs": (c_int, [ctypes.POINTER(LogProbsDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "y3_version": (c_int, []),
     "y3_last_error": (ctypes.c_char_p, []),
 }

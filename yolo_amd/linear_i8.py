@@ -1,0 +1,189 @@
+"""Linear layers and 1x1 convolutions in 8-bit integers, with one scale per row of the input (pixel, token) and one per
+output channel (y3_linear_i8, include/yolo3hip.h):
+
+    layer = Int8Linear(weight, bias, leaky=True)      weight [n, k] float, or int8 with scale=[n]
+    y = layer(x)                                      x [..., k] float32 / bfloat16: rows are quantised on the way
+    rows = quantize_rows(x)                           once, for several layers:
+    y1, y2 = layer1(rows.values, scale=rows.scale), layer2(rows.values, scale=rows.scale)
+
+    y[m, n] = act(s[m] t[n] sum_k q[m, k] w[n, k] + bias[n]),   q = round_half_even(x * (127 / a)),  s = a / 127,
+    a = max(max_k |x_k|, 127 * 2^-126)
+
+The sum is exact, so a row's result does not depend on the rows beside it.  A row with a NaN or an infinity gives NaN.
+`Network(..., int8=True)` runs its 1x1 convolutions this way.  Calls are asynchronous on the current stream of the
+layer's device; nothing is kept from one call for the next, so calls on several streams and in HIP graphs are independent.
+There is no gradient (the package is inference only).
+"""
+import collections
+import contextlib
+import ctypes
+
+import torch
+
+from . import _lib
+
+_CODES = {torch.float32: _lib.Y3_F32, torch.bfloat16: _lib.Y3_BF16, torch.int8: _lib.Y3_I8}
+_NO_GUARD = contextlib.nullcontext()
+
+Int8Rows = collections.namedtuple("Int8Rows", "values scale")
+
+
+def _on(device):
+    """Launches go to the current device: a guard where that is not the tensors' own."""
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _rows_of(x, k, name):
+    """x [..., k] as a matrix whose rows lie at one stride and whose elements are adjacent (copied only if they are not)."""
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError("%s: last dimension must be %d, got shape %r" % (name, k, tuple(x.shape)))
+    if x.dim() != 2:
+        x = x.reshape(-1, k)
+    if (k > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < k):
+        x = x.contiguous()
+    return x
+
+
+def _check_input(x, name):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("%s must be a tensor on the GPU" % name)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient: the 8-bit product has none (use torch.no_grad())" % name)
+
+
+def _repitch(x):
+    """8-bit rows as the kernels read them: on 16 bytes, readable up to a multiple of 16."""
+    rows, k = x.shape
+    pitch = (k + 15) // 16 * 16
+    ld = x.stride(0) if rows > 1 else pitch
+    if x.data_ptr() % 16 == 0 and ld % 16 == 0 and (
+            k == pitch or x.storage_offset() + (rows - 1) * ld + pitch <= x.untyped_storage().nbytes()):
+        return x, ld
+    ld = x.stride(0) if rows > 1 else k
+    q = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
+    _lib.check(_lib.load().y3_quantize_rows_i8(_lib.Y3_I8, x.data_ptr(), rows, k, ld, q.data_ptr(), pitch, None,
+                                               torch.cuda.current_stream(x.device).cuda_stream))
+    return q, pitch
+
+
+def quantize_rows(x):
+    """x [..., k] float32 / bfloat16 -> Int8Rows(values int8 [..., k], scale float32 [...]): values * scale stands for x.
+    The values are a view of rows padded to 16 bytes, which is how Int8Linear reads them without a copy."""
+    _check_input(x, "x")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("quantize_rows: float32 or bfloat16, got %s" % x.dtype)
+    lead, k = x.shape[:-1], x.shape[-1] if x.dim() else 0
+    m = _rows_of(x, k, "x")
+    rows, pitch = m.shape[0], (k + 15) // 16 * 16
+    q = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
+    s = torch.empty(rows, dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        _lib.check(_lib.load().y3_quantize_rows_i8(_CODES[x.dtype], m.data_ptr(), rows, k, m.stride(0) if rows > 1 else k,
+                                                   q.data_ptr(), pitch, s.data_ptr(),
+                                                   torch.cuda.current_stream(x.device).cuda_stream))
+    return Int8Rows(q[:, :k].view(lead + (k,)) if len(lead) == 1 else q.view(lead + (pitch,))[..., :k], s.view(lead))
+
+
+class Int8Linear(object):
+    """weight [n, k]: float32 / bfloat16 (each row quantised here), or int8 with its scale float32 [n].  bias [n] or None.
+    out_dtype torch.bfloat16 (default) or torch.float32; leaky: leaky-ReLU (alpha 0.1) behind the bias."""
+
+    def __init__(self, weight, bias=None, scale=None, leaky=False, out_dtype=torch.bfloat16, device=None):
+        weight = torch.as_tensor(weight)
+        if device is None:
+            device = weight.device if weight.is_cuda else torch.device("cuda", torch.cuda.current_device())
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("Int8Linear needs a GPU, got device %s" % self.device)
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        if weight.dim() != 2 or weight.dtype not in _CODES:
+            raise ValueError("weight must be [n, k] float32, bfloat16 or int8, got %s %r" % (weight.dtype, tuple(weight.shape)))
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("out_dtype must be torch.bfloat16 or torch.float32, got %s" % out_dtype)
+        if (weight.dtype == torch.int8) != (scale is not None):
+            raise ValueError("scale goes with an int8 weight, and only with one")
+        self.n, self.k = int(weight.shape[0]), int(weight.shape[1])
+        self.leaky, self.out_dtype = bool(leaky), out_dtype
+        lib = _lib.load()
+        d = _lib.LinearI8Desc()
+        d.k, d.n = self.k, self.n
+        _lib.check(lib.y3_linear_i8_layout(ctypes.byref(d)))
+        self._k_pad, self._n_pad = d.k_pad, d.n_pad
+        weight = weight.detach().to(self.device).contiguous()
+
+        def vector(v, what):
+            v = torch.as_tensor(v).detach().to(device=self.device, dtype=torch.float32).contiguous()
+            if v.shape != (self.n,):
+                raise ValueError("%s must have shape (%d,), got %r" % (what, self.n, tuple(v.shape)))
+            return v
+
+        self.bias = vector(bias, "bias") if bias is not None else None
+        self.scale = vector(scale, "scale") if scale is not None else torch.empty(self.n, dtype=torch.float32, device=self.device)
+        self._packed = torch.empty(self._k_pad * self._n_pad, dtype=torch.int8, device=self.device)
+        with _on(self.device):
+            _lib.check(lib.y3_linear_i8_pack(ctypes.byref(d), _CODES[weight.dtype], weight.data_ptr(), self.k,
+                                             self._packed.data_ptr(), self.scale.data_ptr(),
+                                             torch.cuda.current_stream(self.device).cuda_stream))
+        self._descs = {}
+        self._weights = (self._packed.data_ptr(), self.scale.data_ptr(), self.bias.data_ptr() if self.bias is not None else None)
+
+    def _desc(self, key):
+        """(descriptor, workspace bytes) of a call's shape."""
+        code, rows, x_ld, out_ld = key
+        d = _lib.LinearI8Desc()
+        d.dtype, d.out_dtype, d.k, d.n, d.rows = code, _CODES[self.out_dtype], self.k, self.n, rows
+        d.x_ld, d.out_ld, d.k_pad, d.n_pad = x_ld, out_ld, self._k_pad, self._n_pad
+        d.flags = _lib.CONV_LEAKY if self.leaky else 0
+        need = ctypes.c_int64(0)
+        _lib.check(_lib.load().y3_linear_i8_workspace_bytes(ctypes.byref(d), ctypes.byref(need)))
+        if len(self._descs) >= 256:         # shapes of a service come and go
+            self._descs.clear()
+        self._descs[key] = hit = (ctypes.byref(d), int(need.value))
+        return hit
+
+    def __call__(self, x, scale=None, out=None):
+        """x [..., k] float32 / bfloat16, or int8 with scale float32 [...].  Returns [..., n] (in `out` if given)."""
+        _check_input(x, "x")
+        if x.device != self.device:
+            raise ValueError("x is on %s, the layer on %s" % (x.device, self.device))
+        code = _CODES.get(x.dtype)
+        if code is None:
+            raise ValueError("x must be float32, bfloat16 or int8, got %s" % x.dtype)
+        if (code == _lib.Y3_I8) != (scale is not None):
+            raise ValueError("scale goes with int8 rows, and only with them")
+        m = _rows_of(x, self.k, "x")
+        rows = m.shape[0]
+        shape = x.shape[:-1] + (self.n,)
+        if out is None:
+            out = torch.empty(shape, dtype=self.out_dtype, device=self.device)
+            out_ld = self.n
+        else:
+            if out.dtype != self.out_dtype or out.shape != shape or out.device != self.device:
+                raise ValueError("out must be %s %r on %s" % (self.out_dtype, tuple(shape), self.device))
+            flat = out.view(-1, self.n) if rows else out            # (a view: rows at one stride, or this raises)
+            out_ld = flat.stride(0) if rows > 1 else self.n
+            if (self.n > 1 and rows and flat.stride(1) != 1) or out_ld < self.n:
+                raise ValueError("out must have adjacent elements in each row and rows that do not overlap")
+        if rows == 0:
+            return out
+        with _on(self.device):
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            scale_ptr = None
+            if code == _lib.Y3_I8:
+                if scale.dtype != torch.float32 or scale.numel() != rows or scale.device != self.device:
+                    raise ValueError("scale must be float32 with one value per row on %s" % self.device)
+                scale = scale.contiguous()
+                scale_ptr = scale.data_ptr()
+                m, x_ld = _repitch(m)
+            else:
+                x_ld = m.stride(0) if rows > 1 else self.k
+            key = (code, rows, x_ld, out_ld)
+            dref, need = self._descs.get(key) or self._desc(key)
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            w, ws_scale, b = self._weights
+            rc = _lib.load().y3_linear_i8(dref, m.data_ptr(), scale_ptr, w, ws_scale, b, out.data_ptr(),
+                                          ws.data_ptr() if need else None, need, stream)
+            if rc:
+                _lib.check(rc)
+        return out
