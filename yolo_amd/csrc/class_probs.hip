@@ -10,6 +10,7 @@
 namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
 constexpr int MAX_TOP = 32;
 
 struct ProbsArgs {
@@ -18,8 +19,10 @@ struct ProbsArgs {
     const void *ids;
     float *logp, *entropy, *top_logp;
     int32_t *top_ids;
-    long rows, group_ld, row_ld, extent;
-    int classes, group, top, ids_64, fast_group;
+    long rows, group_ld, row_ld, extent, first;
+    int classes, group, top, ids_64, fast_group, chunks, chunk_vecs;
+    f32x4 *sums;                       // rows of several chunks: {M, Z, S} and `top` keys per chunk
+    unsigned long long *keys;
     FastDiv fd_group;                  // r / group where fast_group is set (more than one row per group, fewer than 2^31 rows)
 };
 
@@ -84,359 +87,507 @@ template <int L, typename T, typename F> __device__ __forceinline__ T lanes_redu
 
 struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return vmax_raw(a, b); } };      // (NaN: the other one)
 struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct MaxU { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return max(a, b); } };
+struct MinU { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return min(a, b); } };
 struct MinI { __device__ __forceinline__ int operator()(int a, int b) const { return min(a, b); } };
 
-// ---- few classes: L lanes per row, up to E logits in each lane's registers -------------------------------------------
-// One read of the row; each alternative is a maximum over the registers and the lanes, the lowest class that has it, and
-// that logit taken out (NaN: no maximum and no comparison sees it).
+// ---- few classes: L lanes per row, E logits in each lane's registers --------------------------------------------------
+// One read of the row.  The alternatives come from 31-bit keys in ascending order, {how far the logit is below the maximum,
+// class}: fp32 takes the bits of the difference, which the softmax has computed anyway, bf16 the 16 bits of the logit itself.
+// With the previous winner + 1 subtracted, every key that is left keeps its order and the ones taken wrap to the upper half,
+// so a round is one subtraction and half a v_min3_u32 per logit (finding the maximum and its class and taking it out costs
+// four times as much: 1.1 M rows of 80, three alternatives, 188 us that way).  bf16 keys are exact.  fp32 keys that agree in
+// all but the class leave open which logit is larger: one more round shows whether any of the first `top` + 1 do, and the
+// wave then settles its rows with whole logits.
 template <int DT, int L, int E>
 __global__ __launch_bounds__(256) void probs_lanes_kernel(const ProbsArgs p) {
-    constexpr int RPW = 64 / L;
+    constexpr int RPW = 64 / L, SURE = E - 2;                    // the first SURE logits of every lane exist (launch_probs)
+    constexpr unsigned MASK = L * E <= 128 ? 127 : L * E <= 256 ? 255 : L * E <= 512 ? 511 : 1023;
     const int lane = threadIdx.x & 63, l = lane & (L - 1);
-    const long waves = (long)gridDim.x * 4;
     const float nan = __builtin_nanf(""), ninf = -__builtin_inff();
-    for (long r0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW; r0 < p.rows; r0 += waves * RPW) {
-        const long r = r0 + lane / L;
-        const long at = r < p.rows ? row_start(p, r) : -1;
-        if (at < 0) {                                           // (the lanes of a row go together)
-            if (at == -2) put_row_outside(p, r, l, L);
-            continue;
+    const long r = p.first + ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + lane / L;
+    const long at = r < p.rows ? row_start(p, r) : -1;
+    if (at < 0) {                                               // (the lanes of a row go together)
+        if (at == -2) put_row_outside(p, r, l, L);
+        return;
+    }
+    const char *z = p.z + at * (DT == Y3_F32 ? 4 : 2);
+    float x[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = logit<DT>(z, j < SURE ? j * L + l : min(j * L + l, p.classes - 1));
+    long id = -1;
+    float zid = 0.0f;
+    if (p.logp) {
+        id = row_id(p, r);
+        if (id >= 0 && id < p.classes) zid = logit<DT>(z, id);
+    }
+#pragma unroll
+    for (int j = SURE; j < E; ++j) x[j] = j * L + l < p.classes ? x[j] : ninf;
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < E; ++j) m = vmax_raw(m, x[j]);
+    m = lanes_reduce<L>(m, Max());
+    const float m0 = m == ninf ? 0.0f : m;
+    float zs = 0.0f, ss = 0.0f;
+    unsigned k[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        const float d = x[j] - m0, e = __builtin_amdgcn_exp2f(d * LOG2E);
+        zs += e;
+        ss = fmaf(e, vmax_raw(d, -1e4f), ss);               // (an e of 0 adds nothing, whatever d is)
+        if constexpr (DT == Y3_F32) {
+            k[j] = (__float_as_uint(d) & (0x7fffffffu & ~MASK)) | (unsigned)(j * L + l);
+        } else {
+            const unsigned u = __float_as_uint(x[j] + 0.0f);            // (one zero)
+            k[j] = ((((u ^ ~(unsigned)((int)u >> 31)) & 0x7fffffffu) ^ (u & 0x80000000u)) >> 1 & ~MASK) | (unsigned)(j * L + l);
         }
-        const char *z = p.z + at * (DT == Y3_F32 ? 4 : 2);
-        float x[E];
+    }
+    zs = lanes_reduce<L>(zs, Add());
+    ss = lanes_reduce<L>(ss, Add());
+    const bool none = zs == 0.0f, bad = !(zs < __builtin_inff());
+    const float log_z = none ? 0.0f : __builtin_amdgcn_logf(zs) * LN2;
+    if (l == 0) put_scalars(p, r, zid, id, m, log_z, none ? 0.0f : fmaf(-ss, __builtin_amdgcn_rcpf(zs), log_z));
+    if (!p.top) return;
+    const auto put = [&](int t, int c) {                     // alternative t of the row, by one of its lanes
+        p.top_ids[r * p.top + t] = bad ? t : c;
+        p.top_logp[r * p.top + t] = bad ? nan : log_prob(logit<DT>(z, c), m, log_z);
+    };
+    unsigned past = 0, open = 0;                             // the last winner + 1
+    int mine = 0;
+    const int rounds = DT == Y3_F32 ? min(p.top + 1, p.classes) : p.top;
+    for (int t = 0; t < rounds; ++t) {
+        unsigned d = ~0u;
 #pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = j * L + l < p.classes ? logit<DT>(z, j * L + l) : ninf;
-        long id = -1;
-        float zid = 0.0f;
-        if (p.logp) {
-            id = row_id(p, r);
-            if (id >= 0 && id < p.classes) zid = logit<DT>(z, id);
+        for (int j = 0; j < E; ++j) d = min(d, k[j] - past);
+        d = lanes_reduce<L>(d, MinU());
+        const unsigned next = past + d;
+        open |= (unsigned)(t > 0 && (next ^ (past - 1)) <= MASK);
+        past = next + 1;
+        const int c = min((int)(next & MASK), p.classes - 1);               // (NaN rows: any class, not used)
+        if (l == (t & (L - 1))) mine = c;                    // lane t keeps alternative t: rows are stored in one piece
+        if ((t & (L - 1)) == L - 1 || t == rounds - 1) {
+            const int first = t & ~(L - 1);
+            if (first + l < min(t + 1, p.top)) put(first + l, mine);
         }
-        float m = x[0];
+    }
+    if (DT == Y3_F32 && __ballot(open)) {                    // whole logits: the maximum, the lowest class that has it, ...
 #pragma unroll
-        for (int j = 1; j < E; ++j) m = vmax_raw(m, x[j]);
-        m = lanes_reduce<L>(m, Max());
-        const float m0 = m == ninf ? 0.0f : m;
-        float zs = 0.0f, ss = 0.0f;
+        for (int j = 0; j < E; ++j) x[j] = j * L + l < p.classes ? logit<DT>(z, j * L + l) : nan;
+        for (int t = 0; t < p.top; ++t) {
+            float v = x[0];
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const float d = x[j] - m0, e = __builtin_amdgcn_exp2f(d * LOG2E);
-            zs += e;
-            ss = fmaf(e, vmax_raw(d, -1e4f), ss);               // (an e of 0 adds nothing, whatever d is)
-        }
-        zs = lanes_reduce<L>(zs, Add());
-        ss = lanes_reduce<L>(ss, Add());
-        const bool none = zs == 0.0f, bad = !(zs < __builtin_inff());
-        const float log_z = none ? 0.0f : logf(zs);
-        if (l == 0) put_scalars(p, r, zid, id, m, log_z, none ? 0.0f : log_z - ss / zs);
-        if (p.top) {
+            for (int j = 1; j < E; ++j) v = vmax_raw(v, x[j]);
+            v = lanes_reduce<L>(v, Max());
+            int c = 0x7fffffff;
 #pragma unroll
-            for (int j = 0; j < E; ++j) x[j] = j * L + l < p.classes ? x[j] : nan;
-            float keep_lp = 0.0f;
-            int keep_id = 0;
-            for (int t = 0; t < p.top; ++t) {
-                float v = m;
-                if (t) {
-                    v = x[0];
+            for (int j = E - 1; j >= 0; --j) c = x[j] == v ? j * L + l : c;
+            c = lanes_reduce<L>(c, MinI());
 #pragma unroll
-                    for (int j = 1; j < E; ++j) v = vmax_raw(v, x[j]);
-                    v = lanes_reduce<L>(v, Max());
-                }
-                int c = 0x7fffffff;
-#pragma unroll
-                for (int j = E - 1; j >= 0; --j) c = x[j] == v ? j * L + l : c;
-                c = lanes_reduce<L>(c, MinI());
-#pragma unroll
-                for (int j = 0; j < E; ++j) x[j] = c == j * L + l ? nan : x[j];
-                if (l == (t & (L - 1))) {                        // lane t keeps alternative t: rows are stored in one piece
-                    keep_id = bad ? t : c;
-                    keep_lp = bad ? nan : log_prob(v, m, log_z);
-                }
-                if ((t & (L - 1)) == L - 1 || t == p.top - 1) {
-                    const int first = t & ~(L - 1);
-                    if (first + l <= t) {
-                        p.top_ids[r * p.top + first + l] = keep_id;
-                        p.top_logp[r * p.top + first + l] = keep_lp;
-                    }
-                }
-            }
+            for (int j = 0; j < E; ++j) x[j] = c == j * L + l ? nan : x[j];         // ... and that one taken out
+            if (l == 0) put(t, min(c, p.classes - 1));
         }
     }
 }
 
-// ---- many classes: W waves per row ----------------------------------------------------------------------------------
-// One pass with a running maximum per lane (Z and S scaled along with it).  The row is read in 16-byte vectors: vector 0 is
-// what lies in front of the first 16-byte border, the last one what lies behind the last; lane t of the row takes vectors
-// t, t + 64 W, ...  Each lane remembers its largest logit and the vector that has it.  For `top` alternatives the wave's
-// top-th largest of these 64 maxima is a bound T that at least `top` of its logits reach, and only the lanes whose maximum
-// reaches T hold such logits: their vectors alone (top of 64) are read again, from cache, and the logits from T on listed.
-// The bound is a key with the class in it, so equal logits do not swell the list; should it fill up all the same, it is
-// cut to its `top` largest, which raises T.  Waves join through LDS, in a fixed order.
-constexpr int LIST = 192;
+// ---- many classes: rows in chunks of up to 8192 logits, one workgroup of four waves per chunk ---------------------------
+// A chunk is read once, in 16-byte vectors, into registers (vector 0 of a row is what lies in front of its first 16-byte
+// border, the last one what lies behind the last), and everything is done there: the thread's maximum, its sums, and the
+// candidates for the alternatives.  For those, the top-th largest of the 64 quads' maxima (found by bisection of its bits,
+// one ballot each) is a bound that at least `top` logits reach and few others do: those are listed, and ranked by counting
+// the larger keys.  A list that overflows (hundreds of equal logits at the border) is settled by one search per alternative.
+// Rows of more than one chunk leave {M, Z, S} and the chunk's first `top` keys in the workspace for probs_join_kernel, which
+// merges them in a fixed order.  One workgroup walking a whole row instead: 31 us for one row of 128000 (its exponentials
+// alone keep one CU busy for 9 us), 98 us for 4096 rows of 32001.
+constexpr int LIST = 512, CHUNK_THREADS = 256;
 
 typedef unsigned long long u64;
 __device__ __forceinline__ u64 key_of(float x, int c) { return (u64)order_of(x) << 32 | (0xffffffffu - (unsigned)c); }
 
-// LDS is in order within a wave; this keeps the compiler to it (what another lane wrote is read behind it)
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+// Over a whole wave, all lanes active: within 16 lanes as lanes_reduce, then row 0 into 1, 2 into 3, and 1 into 2 and 3; the
+// last lane's value in every lane.  (`none`: what changes nothing.)
+template <typename T, typename F> __device__ __forceinline__ T wave_reduce(T v, T none, F f) {
+    v = lanes_reduce<16>(v, f);
+    const int n = __builtin_bit_cast(int, none);
+    v = f(v, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, false)));
+    v = f(v, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, false)));
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+__device__ __forceinline__ u64 wave_max_u64(u64 v) {
+    const unsigned hi = wave_reduce((unsigned)(v >> 32), 0u, MaxU());
+    const unsigned lo = wave_reduce((unsigned)(v >> 32) == hi ? (unsigned)v : 0u, 0u, MaxU());
+    return (u64)hi << 32 | lo;
 }
 
-// the `top` largest of list[0 .. n) to its front, in order, the rest of the first `top` cleared; returns the last one's key
-__device__ __forceinline__ u64 cut_list(u64 *list, int n, int top, int lane) {
-    u64 k[LIST / 64];
-    int rank[LIST / 64];
-#pragma unroll
-    for (int i = 0; i < LIST / 64; ++i) {
-        k[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0;
-        rank[i] = 0;
-    }
-    for (int s = 0; s < n; ++s) {
-        const u64 o = list[s];
-#pragma unroll
-        for (int i = 0; i < LIST / 64; ++i) rank[i] += o > k[i];
-    }
-    wave_sync();
-    if (lane < top) list[lane] = 0;
-    wave_sync();
-#pragma unroll
-    for (int i = 0; i < LIST / 64; ++i)
-        if (k[i] && rank[i] < top) list[rank[i]] = k[i];
-    wave_sync();
-    return list[top - 1];
+struct Sums { float m, z, s; };
+// scaled to another maximum that is not below (both -inf: the difference is NaN, the factor 0, Z = S = 0)
+__device__ __forceinline__ Sums scaled(Sums a, float m) {
+    const float d = vmax_raw(a.m - m, -1e4f), f = __builtin_amdgcn_exp2f(d * LOG2E);
+    return Sums{m, a.z * f, f * fmaf(d, a.z, a.s)};
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+    const float m = vmax_raw(a.m, b.m);
+    a = scaled(a, m);
+    b = scaled(b, m);
+    return Sums{m, a.z + b.z, a.s + b.s};
+}
+__device__ __forceinline__ Sums wave_join(Sums a) {
+    a = scaled(a, wave_reduce(a.m, -__builtin_inff(), Max()));
+    return Sums{a.m, wave_reduce(a.z, 0.0f, Add()), wave_reduce(a.s, 0.0f, Add())};
 }
 
-template <int DT, int W>
-__global__ __launch_bounds__(64 * W) void probs_row_kernel(const ProbsArgs p) {
-    constexpr int VE = DT == Y3_F32 ? 4 : 8, ES = DT == Y3_F32 ? 4 : 2, STEP = 64 * W, G = 4;
-    __shared__ u64 lists[W][LIST];
-    __shared__ float part[W][3];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+struct Row { float m, log_z, entropy; bool bad; };
+__device__ __forceinline__ Row finish(Sums s) {
+    const bool none = s.z == 0.0f;
+    const float log_z = none ? 0.0f : __builtin_amdgcn_logf(s.z) * LN2;
+    return Row{s.m, log_z, none ? 0.0f : fmaf(-s.s, __builtin_amdgcn_rcpf(s.z), log_z), !(s.z < __builtin_inff())};
+}
+__device__ __forceinline__ void put_alternative(const ProbsArgs &p, long r, int t, u64 k, const Row &w) {
+    p.top_ids[r * p.top + t] = w.bad ? t : (int)(0xffffffffu - (unsigned)k);
+    p.top_logp[r * p.top + t] = w.bad ? __builtin_nanf("") : log_prob(of_order((unsigned)(k >> 32)), w.m, w.log_z);
+}
+// place of a key among list[0 .. n), cleared up to the next multiple of 8
+__device__ __forceinline__ int place_in(const u64 *list, int n, u64 k) {
+    int rank = 0;
+    for (int o = 0; o < n; o += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rank += list[o + i] > k;
+    }
+    return rank;
+}
+
+template <int DT>
+__global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8))) void probs_chunk_kernel(const ProbsArgs p) {
+    constexpr int VE = DT == Y3_F32 ? 4 : 8, ES = DT == Y3_F32 ? 4 : 2, NV = 32 / VE, STEP = CHUNK_THREADS, W = STEP / 64;
+    __shared__ __attribute__((aligned(16))) u64 list[LIST];
+    __shared__ u64 red[W];
+    __shared__ float part[W][3], quads[STEP / 4], bound_s;
+    __shared__ int list_n;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float ninf = -__builtin_inff();
-    u64 *list = lists[wave];
-    for (long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const long at = row_start(p, r);
-        if (at < 0) {
-            if (at == -2) put_row_outside(p, r, threadIdx.x, STEP);
-            continue;
-        }
-        const char *z = p.z + at * ES;
-        const int C = p.classes, head = (int)((16 - ((uintptr_t)z & 15)) & 15) / ES;
-        const int vecs = 1 + (C > head ? (C - head + VE - 1) / VE : 0), whole = 1 + (C > head ? (C - head) / VE : 0);
-        const auto unpack = [&](const u32x4 &v, float (&x)[VE]) {
-            if constexpr (DT == Y3_F32) {
+    const long i = p.first + blockIdx.x;                         // (no loop: what it hoists costs a third of the registers)
+    const long r = p.chunks == 1 ? i : i / p.chunks;
+    const int chunk = (int)(i - r * p.chunks);
+    const long at = row_start(p, r);
+    if (at < 0) {
+        if (at == -2 && chunk == 0) put_row_outside(p, r, tid, STEP);
+        return;
+    }
+    const char *z = p.z + at * ES;
+    const int C = p.classes, top = p.top, head = (int)((16 - ((uintptr_t)z & 15)) & 15) / ES;
+    const int whole = 1 + (C - head) / VE, v0 = chunk * p.chunk_vecs;                    // (C > 1024)
+    const int c0 = max(0, head + (v0 - 1) * VE), c1 = min(C, head + (v0 + p.chunk_vecs - 1) * VE);   // the chunk's classes
+    const auto first_of = [&](int g) { return head + (v0 + tid + g * STEP - 1) * VE; };
+    u32x4 raw[NV];
+    const int w_last = wave * 64 + 63 + (NV - 1) * STEP;      // (wave-uniform: all of its vectors are there and whole)
+    if (v0 + wave * 64 >= 1 && w_last < p.chunk_vecs && v0 + w_last < whole) {
+        const char *zw = z + (long)(head + (v0 + wave * 64 - 1) * VE) * ES;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(v[j]);
-            } else {
+        for (int g = 0; g < NV; ++g) raw[g] = *(const u32x4 *)(zw + (unsigned)(lane * 16 + g * STEP * 16));
+    } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(v[j] << 16); x[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u); }
-            }
-        };
-        const auto first_of = [&](int u) { return head + (u - 1) * VE; };
-        const auto load = [&](int u, float (&x)[VE]) {           // any vector; -inf where the row has nothing
-            const int b = first_of(u);
-            if (u >= 1 && u < whole) unpack(*(const u32x4 *)(z + (long)b * ES), x);
-            else
+        for (int g = 0; g < NV; ++g) {                       // -inf where the chunk has nothing
+            const int in = tid + g * STEP, u = v0 + in, b = first_of(g);
+            raw[g] = DT == Y3_F32 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u} : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+            if (in < p.chunk_vecs) {
+                if (u >= 1 && u < whole) raw[g] = *(const u32x4 *)(z + (unsigned)(b * ES));
+                else if (u <= whole) {
+#pragma unroll 1
+                    for (int j = 0; j < VE; ++j) {           // the vector at an end of the row
+                        if (b + j < 0 || b + j >= C) continue;
+                        const unsigned bits = DT == Y3_F32 ? ((const unsigned *)z)[b + j] : ((const unsigned short *)z)[b + j];
+                        const int word = j * ES / 4, shift = j * ES % 4 * 8;
+                        const unsigned mask = (DT == Y3_F32 ? ~0u : 0xffffu) << shift;
 #pragma unroll
-                for (int j = 0; j < VE; ++j) x[j] = b + j >= 0 && b + j < C ? logit<DT>(z, b + j) : ninf;
-        };
-        float m = ninf, zs = 0.0f, ss = 0.0f, big = ninf;
-        int big_u = threadIdx.x;
-        const auto take = [&](int u, float (&x)[G][VE]) {        // G vectors u, u + STEP, ..
-            float vm[G], gm = ninf;
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                vm[g] = x[g][0];
-#pragma unroll
-                for (int j = 1; j < VE; ++j) vm[g] = vmax_raw(vm[g], x[g][j]);
-                gm = vmax_raw(gm, vm[g]);
-                const bool more = vm[g] > big;
-                big = more ? vm[g] : big;
-                big_u = more ? u + g * STEP : big_u;
-            }
-            const float nm = vmax_raw(m, gm), n0 = nm == ninf ? 0.0f : nm;
-            const float d = vmax_raw(m - nm, -1e4f), f = __builtin_amdgcn_exp2f(d * LOG2E);       // (m = -inf: Z = S = 0, f = 0)
-            ss = f * fmaf(d, zs, ss);
-            zs *= f;
-            m = nm;
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int j = 0; j < VE; ++j) {
-                    const float y = x[g][j] - n0, e = __builtin_amdgcn_exp2f(y * LOG2E);
-                    zs += e;
-                    ss = fmaf(e, vmax_raw(y, -1e4f), ss);        // (an e of 0 adds nothing, whatever y is)
-                }
-        };
-        int u = threadIdx.x;
-        {                                                        // the first group has the head; the body has whole vectors only
-            float x[G][VE];
-#pragma unroll
-            for (int g = 0; g < G; ++g) load(u + g * STEP, x[g]);
-            take(u, x);
-            u += G * STEP;
-        }
-        const int base = wave * 64;                              // (wave-uniform bounds)
-        int ub = base + G * STEP;
-        for (; ub + 63 + (G - 1) * STEP < whole; ub += G * STEP, u += G * STEP) {
-            u32x4 v[G];
-#pragma unroll
-            for (int g = 0; g < G; ++g) v[g] = *(const u32x4 *)(z + (long)first_of(u + g * STEP) * ES);
-            float x[G][VE];
-#pragma unroll
-            for (int g = 0; g < G; ++g) unpack(v[g], x[g]);
-            take(u, x);
-        }
-        for (; ub < vecs; ub += G * STEP, u += G * STEP) {
-            float x[G][VE];
-#pragma unroll
-            for (int g = 0; g < G; ++g) load(u + g * STEP, x[g]);
-            take(u, x);
-        }
-        // the wave's sums
-        {
-            const float wm = lanes_reduce<64>(m, Max());
-            const float d = vmax_raw(m - wm, -1e4f), f = __builtin_amdgcn_exp2f(d * LOG2E);
-            ss = lanes_reduce<64>(f * fmaf(d, zs, ss), Add());
-            zs = lanes_reduce<64>(zs * f, Add());
-            m = wm;
-        }
-        const int top = p.top;
-        if (top) {
-            // this lane's largest logit as a key: the first place in its vector that has it
-            u64 mine = 0;
-            {
-                float x[VE];
-                load(big_u, x);
-                const int b = first_of(big_u);
-#pragma unroll
-                for (int j = VE - 1; j >= 0; --j)
-                    if (x[j] == big && b + j >= 0 && b + j < C) mine = key_of(big, b + j);
-            }
-            list[lane] = mine;
-            wave_sync();
-            int rank = 0;
-            for (int s = 0; s < 64; ++s) rank += list[s] > mine;
-            wave_sync();
-            u64 bound = 0;                                       // 0: fewer than `top` lanes have anything, everything is listed
-            {
-                const u64 has = __ballot(rank == top - 1 && mine != 0);
-                if (has) {
-                    const int at_lane = __builtin_ctzll(has);
-                    bound = (u64)(unsigned)__shfl((int)(mine >> 32), at_lane) << 32 | (unsigned)__shfl((int)mine, at_lane);
-                }
-            }
-            int n = 0;
-            if (top == 1 && bound) {
-                if (lane == 0) list[0] = bound;
-                n = 1;
-            } else {
-                // the lanes that reach the bound, packed into the low lanes (a lane without a key has a bound of 0 beside it)
-                const u64 reach = __ballot(mine >= bound);
-                const int lanes = __popcll(reach);
-                const int place = __popcll(reach & ((1ull << lane) - 1));
-                wave_sync();
-                if (reach >> lane & 1) list[place] = (u64)lane;
-                wave_sync();
-                const int owner = lane < lanes ? (int)list[lane] : 0;      // (kept in a register: the list is filled next)
-                wave_sync();
-                const int per = (vecs - 1 - base + STEP) / STEP;           // vectors of the wave's first lane: the most any has
-                const int items = vecs > base ? lanes * per : 0;
-                for (int q0 = 0; q0 < items; q0 += 64) {
-                    const int q = q0 + lane, o = min(q / per, lanes - 1);
-                    const int uu = base + __shfl(owner, o) + (q - o * per) * STEP;
-                    float x[VE];
-                    const bool on = q < items && uu < vecs;
-                    if (on) load(uu, x);
-                    const int b = first_of(uu);
-#pragma unroll
-                    for (int j = 0; j < VE; ++j) {
-                        const u64 k = on && b + j >= 0 && b + j < C ? key_of(x[j], b + j) : 0;
-                        const bool in = k != 0 && k >= bound;
-                        const u64 set = __ballot(in);
-                        if (set == 0) continue;
-                        if (n + __popcll(set) > LIST) {
-                            const u64 last = cut_list(list, n, top, lane);
-                            n = top;                              // (n > LIST - 64 > 32: there are at least `top`)
-                            bound = last > bound ? last : bound;
-                        }
-                        if (in) list[n + __popcll(set & ((1ull << lane) - 1))] = k;
-                        n += __popcll(set);
-                        wave_sync();
+                        for (int w = 0; w < 4; ++w) raw[g][w] = w == word ? (raw[g][w] & ~mask) | bits << shift : raw[g][w];
                     }
                 }
             }
-            cut_list(list, n, top, lane);
         }
-        if constexpr (W > 1) {
-            if (lane == 0) { part[wave][0] = m; part[wave][1] = zs; part[wave][2] = ss; }
-            __syncthreads();
-            if (top || wave == 0) {
-                float tm = part[0][0];
+    }
+    long id = -1;
+    float zid = 0.0f;
+    if (tid == 0) {
+        if (p.logp && p.chunks == 1) {
+            id = row_id(p, r);
+            if (id >= 0 && id < C) zid = logit<DT>(z, id);
+        }
+        list_n = 0;
+    }
+    if (top > 1) *(u32x4 *)(list + 2 * tid) = u32x4{0, 0, 0, 0};
+    const auto value = [&](int g, int j) {
+        if constexpr (DT == Y3_F32) return __uint_as_float(raw[g][j]);
+        else return __uint_as_float(j % 2 ? raw[g][j / 2] & 0xffff0000u : raw[g][j / 2] << 16);
+    };
+    const auto unseen = [&]() {                              // (bf16 is unpacked again where it is used: half the registers)
 #pragma unroll
-                for (int w = 1; w < W; ++w) tm = vmax_raw(tm, part[w][0]);
-                float tz = 0.0f, ts = 0.0f;
+        for (int g = 0; g < NV; ++g) asm volatile("" : "+v"(raw[g]));
+    };
+    float vmax[NV], big = ninf;
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const float d = vmax_raw(part[w][0] - tm, -1e4f), f = __builtin_amdgcn_exp2f(d * LOG2E);
-                    ts += f * fmaf(d, part[w][1], part[w][2]);
-                    tz += f * part[w][1];
-                }
-                m = tm; zs = tz; ss = ts;
-            }
+    for (int g = 0; g < NV; ++g) {
+        vmax[g] = value(g, 0);
+#pragma unroll
+        for (int j = 1; j < VE; ++j) vmax[g] = vmax_raw(vmax[g], value(g, j));
+        big = vmax_raw(big, vmax[g]);
+    }
+    // exp(x - M) as exp2(x log2 e - fl(M log2 e)), one fused operation: the rounding r of M log2 e is in every exponent
+    // alike and comes out of the sums behind the loop.  That does not hold for magnitudes whose product overflows, and
+    // 0 * -inf makes S a NaN where there are impossible classes: such lanes' waves do it the long way.
+    Sums s = {big, 0.0f, 0.0f};
+    const float ml = big * LOG2E;
+    unseen();
+#pragma unroll
+    for (int g = 0; g < NV; ++g)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const float y = fmaf(value(g, j), LOG2E, -ml), e = __builtin_amdgcn_exp2f(y);
+            s.z += e;
+            s.s = fmaf(e, y, s.s);
         }
-        const bool none = zs == 0.0f, bad = !(zs < __builtin_inff());
-        const float log_z = none ? 0.0f : logf(zs);
-        if (threadIdx.x == 0) {
-            long id = -1;
-            float zid = 0.0f;
-            if (p.logp) {
-                id = row_id(p, r);
-                if (id >= 0 && id < C) zid = logit<DT>(z, id);
+    {
+        const float r = fmaf(big, LOG2E, -ml);
+        s.s = fmaf(-r, s.z, s.s) * LN2;
+        const float f = __builtin_amdgcn_exp2f(-r);
+        s.z *= f;
+        s.s *= f;
+    }
+    if (__ballot(!(fabsf(big) < 1e37f) || s.s != s.s)) {
+        const float m0 = big == ninf ? 0.0f : big;
+        unseen();
+        s.z = s.s = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NV; ++g)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                const float y = value(g, j) - m0, e = __builtin_amdgcn_exp2f(y * LOG2E);
+                s.z += e;
+                s.s = fmaf(e, vmax_raw(y, -1e4f), s.s);      // (an e of 0 adds nothing, whatever y is)
             }
-            put_scalars(p, r, zid, id, m, log_z, none ? 0.0f : log_z - ss / zs);
-        }
+    }
+    s = wave_join(s);
+    const float quad = lanes_reduce<4>(big, Max());
+    if (lane == 0) { part[wave][0] = s.m; part[wave][1] = s.z; part[wave][2] = s.s; }
+    if ((lane & 3) == 0) quads[tid >> 2] = quad;
+    __syncthreads();
+    Row row = {0.0f, 0.0f, 0.0f, false};
+    if (wave == 0) {
         if (top) {
-            // the place of every wave's keys among all: keys are distinct, so counting the larger ones is enough
-            for (int q = threadIdx.x; q < W * top; q += STEP) {
-                const u64 k = lists[q / top][q % top];
-                int rank = 0;
-                if constexpr (W == 1) rank = q;
-                else
-                    for (int w = 0; w < W; ++w)
-                        for (int s = 0; s < top; ++s) rank += lists[w][s] > k;
-                if (bad ? q < top : (k != 0 && rank < top)) {
-                    const int to = bad ? q : rank;
-                    p.top_ids[r * top + to] = bad ? q : (int)(0xffffffffu - (unsigned)k);
-                    p.top_logp[r * top + to] = bad ? __builtin_nanf("") : log_prob(of_order((unsigned)(k >> 32)), m, log_z);
+            unsigned t = 0;
+            const unsigned o = order_of(quads[lane]);
+#pragma unroll
+            for (int b = 31; b >= 0; --b) {
+                const unsigned more = t | 1u << b;
+                t = __popcll(__ballot(o >= more)) >= top ? more : t;
+            }
+            if (lane == 0) bound_s = of_order(t);
+        }
+        s = Sums{part[0][0], part[0][1], part[0][2]};
+#pragma unroll
+        for (int w = 1; w < W; ++w) s = join(s, Sums{part[w][0], part[w][1], part[w][2]});
+        if (p.chunks == 1) {
+            row = finish(s);
+            if (tid == 0) put_scalars(p, r, zid, id, row.m, row.log_z, row.entropy);
+        } else if (tid == 0) p.sums[i] = f32x4{s.m, s.z, s.s, 0.0f};
+    }
+    if (top) {
+        __syncthreads();
+        const float bound = bound_s;
+        if (bound == ninf) {
+            // fewer than `top` quads have a possible class: of the impossible ones the chunk's first are enough
+            for (int c = c0 + tid; c < c1; c += STEP) {
+                const float x = logit<DT>(z, c);
+                if (x > ninf || (x == ninf && c < c0 + top)) {
+                    const int to = atomicAdd(&list_n, 1);    // (the order of the list does not show)
+                    if (to < LIST) list[to] = key_of(x, c);
                 }
             }
+        } else if (big >= bound) {                           // (what fills a chunk up is -inf)
+            unseen();
+#pragma unroll
+            for (int g = 0; g < NV; ++g)
+                if (vmax[g] >= bound) {
+                    int many = 0;
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) many += value(g, j) >= bound;
+                    int to = atomicAdd(&list_n, many);
+#pragma unroll
+                    for (int j = 0; j < VE; ++j)
+                        if (value(g, j) >= bound) {
+                            if (to < LIST) list[to] = key_of(value(g, j), first_of(g) + j);
+                            ++to;
+                        }
+                }
         }
-        if (W > 1) __syncthreads();                              // (the next row writes the lists and the sums again)
-        else wave_sync();
+        __syncthreads();
+        const int n = list_n;
+        const auto put = [&](int t, u64 k) {                 // (by the first wave: it has the row's sums)
+            if (p.chunks == 1) put_alternative(p, r, t, k, row);
+            else p.keys[i * top + t] = k;
+        };
+        if (n <= LIST) {
+            if (wave == 0) {
+                if (row.bad) {
+                    if (lane < top) put(lane, 0);
+                } else {
+                    for (int q = lane; q < n; q += 64) {
+                        const u64 k = list[q];
+                        const int rank = n == 1 ? 0 : place_in(list, n, k);
+                        if (rank < top) put(rank, k);
+                    }
+                    for (int q = n + lane; q < top; q += 64) put(q, 0);        // (NaN in a chunk of several: fewer keys)
+                }
+            }
+        } else {
+            u64 last = ~0ull;
+            for (int t = 0; t < top; ++t) {
+                u64 best = 0;
+                for (int c = c0 + tid; c < c1; c += STEP) {
+                    const u64 k = key_of(logit<DT>(z, c), c);
+                    if (k < last && k > best) best = k;
+                }
+                best = wave_max_u64(best);
+                if (lane == 0) red[wave] = best;
+                __syncthreads();
+                last = red[0];
+#pragma unroll
+                for (int w = 1; w < W; ++w) last = red[w] > last ? red[w] : last;
+                __syncthreads();
+                if (tid == 0) put(t, last);
+            }
+        }
     }
 }
 
+// One workgroup per row: the chunks' sums in order; their keys from the largest `top`-th one on, ranked by counting.
+template <int DT>
+__global__ __launch_bounds__(CHUNK_THREADS) void probs_join_kernel(const ProbsArgs p) {
+    __shared__ __attribute__((aligned(16))) u64 list[LIST];
+    __shared__ u64 red[CHUNK_THREADS / 64];
+    __shared__ int list_n;
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads / 64;
+    for (long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const long at = row_start(p, r);
+        if (at < 0) continue;
+        const int top = p.top, n_keys = p.chunks * top;
+        const u64 *keys = p.keys + r * n_keys;
+        u64 bound = 0;                                           // `top` keys of one chunk reach its last one
+        if (top)
+            for (int c = lane; c < p.chunks; c += 64) {
+                const u64 k = keys[c * top + top - 1];
+                bound = k > bound ? k : bound;
+            }
+        Sums s = {-__builtin_inff(), 0.0f, 0.0f};
+        for (int c = lane; c < p.chunks; c += 64) {
+            const f32x4 v = p.sums[r * p.chunks + c];
+            s = join(s, Sums{v[0], v[1], v[2]});
+        }
+        constexpr int AHEAD = 4;                                 // keys of this thread, requested before they are needed
+        u64 mine[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) mine[j] = tid + j * threads < n_keys ? keys[tid + j * threads] : 0;
+        long id = -1;
+        float zid = 0.0f;
+        if (tid == 0) {
+            list_n = 0;
+            if (p.logp) {
+                id = row_id(p, r);
+                if (id >= 0 && id < p.classes) zid = logit<DT>(p.z + at * (DT == Y3_F32 ? 4 : 2), id);
+            }
+        }
+        if (top)
+            for (int q = tid; q < LIST / 2; q += threads) *(u32x4 *)(list + 2 * q) = u32x4{0, 0, 0, 0};
+        const Row row = finish(wave_join(s));
+        if (tid == 0) put_scalars(p, r, zid, id, row.m, row.log_z, row.entropy);
+        if (top) {
+            bound = wave_max_u64(bound);
+            __syncthreads();
+            if (row.bad) {
+                if (tid < top) put_alternative(p, r, tid, 0, row);
+            } else {
+                const auto take = [&](u64 k) {
+                    if (k != 0 && k >= bound) {
+                        const int to = atomicAdd(&list_n, 1);
+                        if (to < LIST) list[to] = k;
+                    }
+                };
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) take(mine[j]);
+                for (int q = tid + AHEAD * threads; q < n_keys; q += threads) take(keys[q]);
+                __syncthreads();
+                const int n = list_n;
+                if (n <= LIST) {
+                    for (int q = tid; q < n; q += threads) {
+                        const u64 k = list[q];
+                        const int rank = place_in(list, n, k);
+                        if (rank < top) put_alternative(p, r, rank, k, row);
+                    }
+                } else {
+                    u64 last = ~0ull;
+                    for (int t = 0; t < top; ++t) {
+                        u64 best = 0;
+                        for (int q = tid; q < n_keys; q += threads) {
+                            const u64 k = keys[q];
+                            if (k < last && k > best) best = k;
+                        }
+                        best = wave_max_u64(best);
+                        if (lane == 0) red[wave] = best;
+                        __syncthreads();
+                        last = red[0];
+                        for (int w = 1; w < waves; ++w) last = red[w] > last ? red[w] : last;
+                        __syncthreads();
+                        if (tid == 0) put_alternative(p, r, t, last, row);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Rows of more than 1024 classes: equal chunks of at most 32 logits per thread.
+struct Chunks { int n, vecs; };
+Chunks chunks_of(const y3_log_probs_desc *d) {
+    if (d->classes <= 1024) return Chunks{0, 0};
+    const int ve = d->dtype == Y3_F32 ? 4 : 8, most = CHUNK_THREADS * 32 / ve;
+    const int vecs = 1 + (d->classes + ve - 1) / ve;             // (the most an alignment makes of a row)
+    const int n = (vecs + most - 1) / most;
+    return Chunks{n, (vecs + n - 1) / n};
+}
+
 template <int DT, int L, int E> void launch_lanes(const ProbsArgs &a, hipStream_t st) {
-    const long waves = (a.rows + 64 / L - 1) / (64 / L), blocks = (waves + 3) / 4;
-    hipLaunchKernelGGL((probs_lanes_kernel<DT, L, E>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st, a);
+    constexpr long RPB = 4 * (64 / L), MOST = RPB << 23;         // rows of a block, of a grid (fewer than 2^32 threads)
+    ProbsArgs b = a;
+    for (b.first = 0; b.first < a.rows; b.first += MOST) {
+        const long n = a.rows - b.first < MOST ? a.rows - b.first : MOST;
+        hipLaunchKernelGGL((probs_lanes_kernel<DT, L, E>), dim3((unsigned)((n + RPB - 1) / RPB)), dim3(256), 0, st, b);
+    }
 }
-template <int DT, int W> void launch_row(const ProbsArgs &a, hipStream_t st) {
-    hipLaunchKernelGGL((probs_row_kernel<DT, W>), dim3((unsigned)(a.rows < 65536 ? a.rows : 65536)), dim3(64 * W), 0, st, a);
+// L lanes with E = 2, 4, .. logits each such that all but each lane's last two exist
+template <int DT, int L, int E> void launch_even(const ProbsArgs &a, hipStream_t st) {
+    if constexpr (E < 16)
+        if (a.classes > L * E) return launch_even<DT, L, E + 2>(a, st);
+    launch_lanes<DT, L, E>(a, st);
 }
-template <int DT> void launch_probs(const ProbsArgs &a, hipStream_t st) {
+template <int DT> int launch_probs(const ProbsArgs &a, hipStream_t st) {
     const int C = a.classes;
-    if (C <= 32) launch_lanes<DT, 8, 4>(a, st);
-    else if (C <= 64) launch_lanes<DT, 8, 8>(a, st);
-    else if (C <= 80) launch_lanes<DT, 8, 10>(a, st);
-    else if (C <= 128) launch_lanes<DT, 8, 16>(a, st);
-    else if (C <= 256) launch_lanes<DT, 16, 16>(a, st);
-    else if (C <= 512) launch_lanes<DT, 32, 16>(a, st);
-    else if (C <= 1024) launch_lanes<DT, 64, 16>(a, st);
-    else if (a.rows <= 256 && C > 8192) launch_row<DT, 16>(a, st);
-    else if (a.rows <= 2048 || C > 8192) launch_row<DT, 4>(a, st);
-    else launch_row<DT, 1>(a, st);
+    if (C <= 128) launch_even<DT, 8, 2>(a, st);
+    else if (C <= 256) launch_even<DT, 16, 10>(a, st);
+    else if (C <= 512) launch_even<DT, 32, 10>(a, st);
+    else if (C <= 1024) launch_even<DT, 64, 10>(a, st);
+    else {
+        ProbsArgs c = a;
+        for (c.first = 0; c.first < a.rows * a.chunks; c.first += 1 << 23) {        // (a grid holds fewer than 2^32 threads)
+            const long n = a.rows * a.chunks - c.first;
+            hipLaunchKernelGGL(probs_chunk_kernel<DT>, dim3((unsigned)(n < (1 << 23) ? n : 1 << 23)), dim3(CHUNK_THREADS), 0, st, c);
+        }
+        if (a.chunks == 1) return y3_check_launch("log_probs");
+        const int rc = y3_check_launch("log_probs (chunks)");
+        if (rc) return rc;
+        // one wave where its lanes hold all keys twice over
+        const int threads = a.chunks * a.top <= 128 ? 64 : CHUNK_THREADS;
+        hipLaunchKernelGGL(probs_join_kernel<DT>, dim3((unsigned)(a.rows < (1 << 20) ? a.rows : 1 << 20)), dim3(threads), 0, st, a);
+    }
+    return y3_check_launch("log_probs");
 }
 
 int check_desc(const y3_log_probs_desc *d) {
@@ -455,7 +606,8 @@ extern "C" int y3_log_probs_workspace_bytes(const y3_log_probs_desc *d, int64_t 
     const int rc = check_desc(d);
     if (rc) return rc;
     Y3_REQUIRE(bytes, Y3_E_INVALID, "log_probs: null pointer");
-    *bytes = 0;
+    const Chunks c = chunks_of(d);
+    *bytes = c.n > 1 ? d->rows * c.n * (16 + 8 * (int64_t)d->top) : 0;
     return Y3_OK;
 }
 
@@ -486,7 +638,9 @@ extern "C" int y3_log_probs(const y3_log_probs_desc *d, const void *logits, cons
     a.classes = d->classes; a.group = d->group; a.top = d->top; a.ids_64 = d->ids_64 != 0;
     if (!row_offsets && d->group > 1 && d->rows < 0x7fffffff) a.fd_group = make_fastdiv(d->group);
     a.fast_group = !row_offsets && d->group > 1 && d->rows < 0x7fffffff;
-    if (d->dtype == Y3_F32) launch_probs<Y3_F32>(a, (hipStream_t)stream);
-    else launch_probs<Y3_BF16>(a, (hipStream_t)stream);
-    return y3_check_launch("log_probs");
+    const Chunks c = chunks_of(d);
+    a.chunks = c.n; a.chunk_vecs = c.vecs;
+    a.sums = (f32x4 *)workspace;
+    a.keys = (unsigned long long *)((char *)workspace + d->rows * c.n * 16);
+    return d->dtype == Y3_F32 ? launch_probs<Y3_F32>(a, (hipStream_t)stream) : launch_probs<Y3_BF16>(a, (hipStream_t)stream);
 }
