@@ -277,22 +277,22 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     const int whole = 1 + (C - head) / VE, v0 = chunk * p.chunk_vecs;                    // (C > 1024)
     const int c0 = max(0, head + (v0 - 1) * VE), c1 = min(C, head + (v0 + p.chunk_vecs - 1) * VE);   // the chunk's classes
     const auto first_of = [&](int g) { return head + (v0 + tid + g * STEP - 1) * VE; };
+    // What a chunk does not fill holds -1e38: its exponential is 0 beside any logit above -1e37, and no NaN comes of it.
+    constexpr unsigned FILL = DT == Y3_F32 ? 0xfe960000u : 0xfe96fe96u;
     u32x4 raw[NV];
-    const int w_last = wave * 64 + 63 + (NV - 1) * STEP;      // (wave-uniform: all of its vectors are there and whole)
-    if (v0 + wave * 64 >= 1 && w_last < p.chunk_vecs && v0 + w_last < whole) {
-        const char *zw = z + (long)(head + (v0 + wave * 64 - 1) * VE) * ES;
 #pragma unroll
-        for (int g = 0; g < NV; ++g) raw[g] = *(const u32x4 *)(zw + (unsigned)(lane * 16 + g * STEP * 16));
-    } else {
-#pragma unroll
-        for (int g = 0; g < NV; ++g) {                       // -inf where the chunk has nothing
+    for (int g = 0; g < NV; ++g) {
+        raw[g] = u32x4{FILL, FILL, FILL, FILL};
+        const int w0 = wave * 64 + g * STEP;                     // (wave-uniform: all 64 vectors are there and whole)
+        if (v0 + w0 >= 1 && w0 + 63 < p.chunk_vecs && v0 + w0 + 63 < whole) {
+            raw[g] = *(const u32x4 *)(z + (long)(head + (v0 + w0 - 1) * VE) * ES + lane * 16);
+        } else if (w0 < p.chunk_vecs && v0 + w0 <= whole) {
             const int in = tid + g * STEP, u = v0 + in, b = first_of(g);
-            raw[g] = DT == Y3_F32 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u} : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
             if (in < p.chunk_vecs) {
                 if (u >= 1 && u < whole) raw[g] = *(const u32x4 *)(z + (unsigned)(b * ES));
                 else if (u <= whole) {
 #pragma unroll 1
-                    for (int j = 0; j < VE; ++j) {           // the vector at an end of the row
+                    for (int j = 0; j < VE; ++j) {               // the vector at an end of the row
                         if (b + j < 0 || b + j >= C) continue;
                         const unsigned bits = DT == Y3_F32 ? ((const unsigned *)z)[b + j] : ((const unsigned short *)z)[b + j];
                         const int word = j * ES / 4, shift = j * ES % 4 * 8;
@@ -332,7 +332,8 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     }
     // exp(x - M) as exp2(x log2 e - fl(M log2 e)), one fused operation: the rounding r of M log2 e is in every exponent
     // alike and comes out of the sums behind the loop.  That does not hold for magnitudes whose product overflows, and
-    // 0 * -inf makes S a NaN where there are impossible classes: such lanes' waves do it the long way.
+    // 0 * -inf makes S a NaN where there are impossible classes: such waves, and those with lanes that got nothing or only
+    // logits below -1e37, do it the long way.
     Sums s = {big, 0.0f, 0.0f};
     const float ml = big * LOG2E;
     unseen();
@@ -352,16 +353,26 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
         s.s *= f;
     }
     if (__ballot(!(fabsf(big) < 1e37f) || s.s != s.s)) {
+        const auto real = [&](int g, int j) {
+            const int c = first_of(g) + j;
+            return c >= c0 && c < c1 && tid + g * STEP < p.chunk_vecs ? value(g, j) : ninf;
+        };
+        unseen();
+        big = ninf;
+#pragma unroll
+        for (int g = 0; g < NV; ++g)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) big = vmax_raw(big, real(g, j));
         const float m0 = big == ninf ? 0.0f : big;
         unseen();
-        s.z = s.s = 0.0f;
+        s = Sums{big, 0.0f, 0.0f};
 #pragma unroll
         for (int g = 0; g < NV; ++g)
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
-                const float y = value(g, j) - m0, e = __builtin_amdgcn_exp2f(y * LOG2E);
+                const float y = real(g, j) - m0, e = __builtin_amdgcn_exp2f(y * LOG2E);
                 s.z += e;
-                s.s = fmaf(e, vmax_raw(y, -1e4f), s.s);      // (an e of 0 adds nothing, whatever y is)
+                s.s = fmaf(e, vmax_raw(y, -1e4f), s.s);          // (an e of 0 adds nothing, whatever y is)
             }
     }
     s = wave_join(s);
@@ -392,16 +403,17 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     if (top) {
         __syncthreads();
         const float bound = bound_s;
-        if (bound == ninf) {
-            // fewer than `top` quads have a possible class: of the impossible ones the chunk's first are enough
+        if (bound < -1e37f) {
+            // from memory, where nothing is filled up; of impossible classes the chunk's first are enough (that is when
+            // fewer than `top` quads have a possible one)
             for (int c = c0 + tid; c < c1; c += STEP) {
                 const float x = logit<DT>(z, c);
-                if (x > ninf || (x == ninf && c < c0 + top)) {
+                if (x >= bound && (x != ninf || c < c0 + top)) {
                     const int to = atomicAdd(&list_n, 1);    // (the order of the list does not show)
                     if (to < LIST) list[to] = key_of(x, c);
                 }
             }
-        } else if (big >= bound) {                           // (what fills a chunk up is -inf)
+        } else if (big >= bound) {
             unseen();
 #pragma unroll
             for (int g = 0; g < NV; ++g)
@@ -551,7 +563,8 @@ Chunks chunks_of(const y3_log_probs_desc *d) {
     const int ve = d->dtype == Y3_F32 ? 4 : 8, most = CHUNK_THREADS * 32 / ve;
     const int vecs = 1 + (d->classes + ve - 1) / ve;             // (the most an alignment makes of a row)
     const int n = (vecs + most - 1) / most;
-    return Chunks{n, (vecs + n - 1) / n};
+    // (a multiple of the threads: all of them have the same number of vectors, but for the end of a row)
+    return Chunks{n, ((vecs + n - 1) / n + CHUNK_THREADS - 1) / CHUNK_THREADS * CHUNK_THREADS};
 }
 
 template <int DT, int L, int E> void launch_lanes(const ProbsArgs &a, hipStream_t st) {
