@@ -61,6 +61,45 @@ __device__ __forceinline__ unsigned amax8(const unsigned (&v)[8], unsigned m) {
 }
 
 struct RowScale { float s, inv; bool finite; };
+__device__ __forceinline__ RowScale row_scale(unsigned amax_bits);
+__device__ __forceinline__ unsigned q4(unsigned a, unsigned b, unsigned c, unsigned d, float inv);
+
+// ---- the same eight elements as they are stored (registers are what a kernel that keeps many of them is short of) -------
+template <int DT> struct Raw;
+template <> struct Raw<Y3_BF16> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void load(const char *row, int k0, int left, unsigned (&v)[4]) {
+        const unsigned short *p = (const unsigned short *)row + k0;
+        if (left >= 8) {
+            const u32x4 r = *(const u32x4_u2 *)p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = r[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (2 * j < left ? p[2 * j] : 0u) | (2 * j + 1 < left ? (unsigned)p[2 * j + 1] << 16 : 0u);
+        }
+    }
+    static __device__ __forceinline__ unsigned amax(const unsigned (&v)[4]) {      
+        unsigned m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, max(v[j] << 16 & 0x7fffffffu, v[j] & 0x7fff0000u));
+        return m;
+    }
+    static __device__ __forceinline__ unsigned long long quantize(const unsigned (&v)[4], float inv) {
+        const unsigned lo = q4(v[0] << 16, v[0] & 0xffff0000u, v[1] << 16, v[1] & 0xffff0000u, inv);
+        const unsigned hi = q4(v[2] << 16, v[2] & 0xffff0000u, v[3] << 16, v[3] & 0xffff0000u, inv);
+        return (unsigned long long)hi << 32 | lo;
+    }
+};
+template <> struct Raw<Y3_F32> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void load(const char *row, int k0, int left, unsigned (&v)[8]) { Chunk<Y3_F32>::load(row, k0, left, v); }
+    static __device__ __forceinline__ unsigned amax(const unsigned (&v)[8]) { return amax8(v, 0); }
+    static __device__ __forceinline__ unsigned long long quantize(const unsigned (&v)[8], float inv) {
+        return (unsigned long long)q4(v[4], v[5], v[6], v[7], inv) << 32 | q4(v[0], v[1], v[2], v[3], inv);
+    }
+};
+
 __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
     RowScale r;
     r.finite = amax_bits < 0x7f800000u;
@@ -174,29 +213,29 @@ __global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld,
 
 // ---- the product ------------------------------------------------------------------------------------------------
 struct LinArgs {
-    const char *x;                     // 8-bit rows, 16-byte pitch and alignment
-    const float *x_scale;
+    const char *x;                     // 8-bit rows on 16 bytes, or float rows
+    const float *x_scale;              // with 8-bit rows
     const char *w;
     const float *w_scale, *bias;       // bias may be null
     char *out;
     long rows, x_ld, out_ld;
-    int k16, n, kb;                    // k rounded up to 16 (bytes of a row that may be read), channels, 64-deep k-blocks
-    int leaky, n_blocks;
+    int k, k16, n, kb;                 // k rounded up to 16 (bytes of an 8-bit row that may be read), channels, 64-deep k-blocks
+    int leaky, out_f32;
+    int n_groups, wk, slab;            // panel kernel: workgroups along n, waves along k, k-blocks of a slab
+    FastDiv fd_items;
 };
 
-// four channels nl .. nl + 3 of one row
-template <int OUT>
-__device__ __forceinline__ void store4(const LinArgs &p, long row, int nl, const i32x4 &acc, float s) {
+// four channels of one row: scaled, activated, stored.  t, b: the channels' scales and biases.
+__device__ __forceinline__ void store4(const LinArgs &p, long row, int nl, const i32x4 &acc, float s, const f32x4 &t, const f32x4 &b) {
     if (row >= p.rows || nl >= p.n) return;
     const bool full = nl + 4 <= p.n;
     float y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int c = full ? nl + j : min(nl + j, p.n - 1);
-        y[j] = fmaf((float)acc[j] * p.w_scale[c], s, p.bias ? p.bias[c] : 0.0f);
-        if (p.leaky) y[j] = y[j] > 0.0f ? y[j] : 0.1f * y[j];
+        y[j] = fmaf((float)acc[j] * t[j], s, b[j]);
+        if (p.leaky) y[j] = y[j] > 0.0f ? y[j] : 0.1f * y[j];          // (NaN: the product keeps it)
     }
-    if constexpr (OUT == Y3_F32) {
+    if (p.out_f32) {
         float *o = (float *)p.out + row * p.out_ld + nl;
         if (full) *(f32x4_u4 *)o = f32x4{y[0], y[1], y[2], y[3]};
         else
@@ -209,36 +248,257 @@ __device__ __forceinline__ void store4(const LinArgs &p, long row, int nl, const
     }
 }
 
-// Four waves per workgroup, each 16 rows x 64 channels, everything straight from global memory.
-template <int OUT>
-__global__ __launch_bounds__(256) void linear_i8_kernel(const LinArgs p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int nb = blockIdx.x % p.n_blocks;
-    const long m0 = ((long)(blockIdx.x / p.n_blocks) * 4 + wave) * 16;
-    if (m0 >= p.rows) return;
-    const long row = m0 + (lane & 15), rr = row < p.rows ? row : p.rows - 1;
-    const char *xr = p.x + rr * p.x_ld;
-    const int frags = (p.n + 15) / 16;
-    i32x4 acc[4] = {};
-    for (int kb = 0; kb < p.kb; ++kb) {
-        const int k0 = kb * 64 + (lane >> 4) * 16;
-        i32x4 xf = {};
-        if (k0 < p.k16) xf = *(const i32x4 *)(xr + k0);
+// Panel kernel: a workgroup of eight waves takes 16 RT rows and 16 NT WN channels (WN WK = 8: WN waves side by side along the
+// channels, WK along k).  The rows' 8-bit values are in LDS -- quantised there from float rows, all of k at once, or copied
+// from 8-bit rows in slabs of k -- and every wave reads its weights as whole fragments straight into registers, two
+// groups of eight ahead: weights are used by one wave each, LDS would only add a copy.
+//   LDS: rows on a pitch of 32 bytes more than their length (16 rows on 16 different 16-byte slots), then per row its scale,
+//   per channel its scale and bias; the area of the rows is used again for the sums of the waves along k.
+constexpr int PN_THREADS = 512, PN_WAVES = 8;
+constexpr int PN_LDS_MAX = 160 * 1024;
+
+template <int XT, int RT, int NT>
+__global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(4)))
+void linear_i8_panel_kernel(const LinArgs p) {
+    constexpr int BM = 16 * RT, U = NT == 1 ? 4 : NT == 2 ? 2 : 1;       // U: k-blocks of a group of weight fragments
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int frow = lane & 15, fq = lane >> 4;
+    const int wn_count = PN_WAVES / p.wk, wn = wave % wn_count, wk = wave / wn_count;
+    const int pitch = p.slab * 64 + 32;
+    const int cols = 16 * NT * wn_count;                         // channels of the workgroup
+    const long m0 = (long)(blockIdx.x / p.n_groups) * BM;
+    const int n0 = (int)(blockIdx.x % p.n_groups) * cols;
+    const int nr = (int)(p.rows - m0 < BM ? p.rows - m0 : BM);   // rows that are there
+    const int area = max(BM * pitch, p.wk > 1 ? PN_WAVES * RT * NT * 1024 : 0);
+    float *row_s = (float *)(smem + area), *row_inv = row_s + BM, *col_t = row_inv + BM, *col_b = col_t + cols;
+    unsigned *row_max = (unsigned *)row_inv;
+
+    const int frags = (p.n + 15) >> 4;
+    const char *wp[NT];                                          // this wave's fragments (past the last channel: the last one's)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (nb * 4 + i >= frags) break;
-            const i32x4 wf = *(const i32x4 *)(p.w + (((long)(nb * 4 + i) * p.kb + kb) * 64 + lane) * 16);
-            acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, xf, acc[i], 0, 0, 0);
+    for (int i = 0; i < NT; ++i) wp[i] = p.w + (long)min((n0 >> 4) + wn * NT + i, frags - 1) * p.kb * 1024;
+    const unsigned w_lane = lane * 16;
+
+    for (int c = tid; c < cols; c += PN_THREADS) {
+        const int ch = min(n0 + c, p.n - 1);
+        col_t[c] = p.w_scale[ch];
+        col_b[c] = p.bias ? p.bias[ch] : 0.0f;
+    }
+    if constexpr (XT == Y3_I8) {
+        if (tid < BM) row_s[tid] = p.x_scale[min(m0 + tid, p.rows - 1)];
+    } else {
+        // float rows -> 8-bit rows: chunks of eight values; sixteen neighbouring lanes always share a row
+        constexpr int NI = XT == Y3_BF16 ? 16 : 8;               // chunks a thread keeps between the two looks at them
+        const int per_row = p.kb * 8, items = nr * per_row;
+        const char *x0 = p.x + m0 * p.x_ld * (XT == Y3_BF16 ? 2 : 4);
+        if (tid < BM) row_max[tid] = 0;
+        __syncthreads();
+        const auto at = [&](int item, int &row, int &k0) {
+            row = fast_div(item, p.fd_items);
+            k0 = (item - row * per_row) * 8;
+        };
+        const auto fetch = [&](int item, unsigned (&v)[Raw<XT>::N]) {
+            int row, k0;
+            at(item, row, k0);
+            Raw<XT>::load(x0 + row * p.x_ld * (XT == Y3_BF16 ? 2 : 4), k0, p.k - k0, v);
+        };
+        const auto look = [&](int item, const unsigned (&v)[Raw<XT>::N]) {
+            int row, k0;
+            at(item, row, k0);
+            unsigned m = Raw<XT>::amax(v);
+            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));
+            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));
+            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));
+            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xf, 0xf, false));
+            if (frow == 0) atomicMax(&row_max[row], m);
+        };
+        const auto write = [&](int item, const unsigned (&v)[Raw<XT>::N]) {
+            int row, k0;
+            at(item, row, k0);
+            const float inv = row_inv[row];
+            *(unsigned long long *)(smem + row * pitch + k0) = inv > 0.0f ? Raw<XT>::quantize(v, inv) : 0;
+        };
+        const bool keep = items <= NI * PN_THREADS;
+        unsigned v[NI][Raw<XT>::N];
+        for (int g = 0; g < items; g += NI * PN_THREADS) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                if (g + i * PN_THREADS + tid < items) fetch(g + i * PN_THREADS + tid, v[i]);
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                if (g + i * PN_THREADS + tid < items) look(g + i * PN_THREADS + tid, v[i]);
+        }
+        __syncthreads();
+        if (tid < BM) {
+            const RowScale r = row_scale(row_max[tid]);
+            row_s[tid] = r.s;
+            row_inv[tid] = r.finite ? r.inv : -1.0f;
+        }
+        __syncthreads();
+        for (int g = 0; g < items; g += NI * PN_THREADS) {
+            if (!keep) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    if (g + i * PN_THREADS + tid < items) fetch(g + i * PN_THREADS + tid, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                if (g + i * PN_THREADS + tid < items) write(g + i * PN_THREADS + tid, v[i]);
         }
     }
-    const float s = p.x_scale[rr];
+
+    i32x4 acc[RT][NT] = {};
+    const char *xl[RT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store4<OUT>(p, row, (nb * 4 + i) * 16 + (lane >> 4) * 4, acc[i], s);
+    for (int r = 0; r < RT; ++r) xl[r] = smem + min(r * 16 + frow, nr - 1) * pitch + fq * 16;
+    for (int s0 = 0; s0 < p.kb; s0 += p.slab) {
+        const int s_kb = min(p.slab, p.kb - s0);                 // k-blocks of this slab
+        // this wave's: wk, wk + WK, ...
+        const int mine = s_kb > wk ? (s_kb - wk + p.wk - 1) / p.wk : 0;
+        i32x4 wf[2][U][NT];
+        const auto weights = [&](int g, i32x4 (&f)[U][NT]) {     // group g (past the end: any fragment, not multiplied)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long kb = min(s0 + wk + (g * U + u) * p.wk, p.kb - 1);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) f[u][i] = *(const i32x4 *)(wp[i] + kb * 1024 + w_lane);
+            }
+        };
+        weights(0, wf[0]);
+        if constexpr (XT == Y3_I8) {
+            if (s0) __syncthreads();                             // (the previous slab has been read)
+            const int chunks = s_kb * 4;                         // 16 bytes each
+            for (int i = tid; i < nr * chunks; i += PN_THREADS) {
+                const int row = i / chunks, c = i - row * chunks, k0 = s0 * 64 + c * 16;
+                u32x4 v = {0, 0, 0, 0};
+                if (k0 < p.k16) v = *(const u32x4 *)(p.x + (m0 + row) * p.x_ld + k0);
+                *(u32x4 *)(smem + row * pitch + c * 16) = v;
+            }
+        }
+        __syncthreads();
+        const auto multiply = [&](int g, const i32x4 (&f)[U][NT]) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (g * U + u >= mine) break;
+                const int kb = wk + (g * U + u) * p.wk;
+                i32x4 xf[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) xf[r] = *(const i32x4 *)(xl[r] + kb * 64);
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[r][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[u][i], xf[r], acc[r][i], 0, 0, 0);
+            }
+        };
+        const int groups = (mine + U - 1) / U;
+        for (int g = 0; g < groups; g += 2) {
+            if (g + 1 < groups) weights(g + 1, wf[1]);
+            multiply(g, wf[0]);
+            if (g + 1 < groups) {
+                if (g + 2 < groups) weights(g + 2, wf[0]);
+                multiply(g + 1, wf[1]);
+            }
+        }
+    }
+
+    const auto put = [&](int r, int c, const i32x4 &v) {         // 16 x 16 block: rows r .. r + 15, channels c .. c + 15 of the workgroup's
+        store4(p, m0 + r + frow, n0 + c + fq * 4, v, row_s[r + frow], *(const f32x4 *)(col_t + c + fq * 4), *(const f32x4 *)(col_b + c + fq * 4));
+    };
+    if (p.wk == 1) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) put(r * 16, (wn * NT + i) * 16, acc[r][i]);
+    } else {
+        __syncthreads();                                         // (the rows have been read)
+        i32x4 *sums = (i32x4 *)smem;                             // [wave][r][i][lane]
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sums[((wave * RT + r) * NT + i) * 64 + lane] = acc[r][i];
+        __syncthreads();
+        for (int b = wave; b < wn_count * RT * NT; b += PN_WAVES) {          // block b = (wn, r, i)
+            const int bw = b / (RT * NT), ri = b % (RT * NT);
+            i32x4 v = sums[(bw * RT * NT + ri) * 64 + lane];
+            for (int k = 1; k < p.wk; ++k) v += sums[((k * wn_count + bw) * RT * NT + ri) * 64 + lane];
+            put(ri / NT * 16, (bw * NT + ri % NT) * 16, v);
+        }
+    }
+}
+
+int panel_area(int rt, int nt, int wk, int slab) {
+    const int rows = 16 * rt * (slab * 64 + 32), sums = wk > 1 ? PN_WAVES * rt * nt * 1024 : 0;
+    return rows > sums ? rows : sums;
+}
+int panel_lds(int rt, int nt, int wk, int slab) { return panel_area(rt, nt, wk, slab) + (2 * 16 * rt + 2 * 16 * nt * (PN_WAVES / wk)) * 4; }
+
+template <int XT, int RT, int NT>
+int launch_panel_as(LinArgs a, hipStream_t st) {
+    static thread_local int attr_dev = -1;
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (attr_dev != dev) {
+        if (hipFuncSetAttribute((const void *)linear_i8_panel_kernel<XT, RT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, PN_LDS_MAX) != hipSuccess) {
+            y3_set_error("linear_i8: cannot reserve %d bytes of LDS", PN_LDS_MAX);
+            return Y3_E_LAUNCH;
+        }
+        attr_dev = dev;
+    }
+    const int cols = 16 * NT * (PN_WAVES / a.wk);
+    a.n_groups = (a.n + cols - 1) / cols;
+    const long grid = (a.rows + 16 * RT - 1) / (16 * RT) * a.n_groups;
+    Y3_REQUIRE(grid < (1 << 23), Y3_E_INVALID, "linear_i8: grid of %ld workgroups", grid);
+    hipLaunchKernelGGL((linear_i8_panel_kernel<XT, RT, NT>), dim3((unsigned)grid), dim3(PN_THREADS), panel_lds(RT, NT, a.wk, a.slab), st, a);
+    return y3_check_launch("linear_i8");
+}
+
+struct Panel { int rt, nt, wk, slab; };
+int panel_fit(int bm) { return (PN_LDS_MAX - 6 * 1024) / bm / 64 - 1; }       // k-blocks of bm rows that LDS holds
+template <int XT> int launch_panel(const LinArgs &a, const Panel &c, hipStream_t st) {
+    LinArgs b = a;
+    b.wk = c.wk;
+    b.slab = c.slab;
+    b.fd_items = make_fastdiv(a.kb * 8);
+    if (c.rt == 1) return launch_panel_as<XT, 1, 1>(b, st);
+    if (c.rt == 2) return launch_panel_as<XT, 2, 1>(b, st);
+    if (c.nt == 1) return launch_panel_as<XT, 4, 1>(b, st);
+    if (c.nt == 2) return launch_panel_as<XT, 4, 2>(b, st);
+    return launch_panel_as<XT, 4, 4>(b, st);
+}
+
+// The largest block of rows and channels that still gives every CU a workgroup (weights are read once per 16 RT rows,
+// rows once per 16 NT WN channels); few rows: 16, with the waves along k.
+Panel panel_of(long rows, int n, int kb, bool eight_bit, long cus) {
+    static const Panel all[] = {{4, 4, 1, 0}, {4, 2, 1, 0}, {4, 1, 1, 0}, {2, 1, 1, 0}, {2, 1, 2, 0}, {1, 1, 2, 0}, {1, 1, 4, 0}, {1, 1, 8, 0}};
+    Panel best = {0, 0, 0, 0};
+    for (const Panel &c : all) {
+        const int bm = 16 * c.rt, cols = 16 * c.nt * (PN_WAVES / c.wk);
+        if (c.nt > 1 && n <= cols / 2) continue;                 // half of the waves would have nothing
+        if (c.rt > 1 && rows <= bm / 2) continue;
+        if (c.wk > kb) continue;
+        Panel t = c;
+        t.slab = kb;
+        if (eight_bit) {
+            const int most = 64 * 1024 / bm / 64;                // (two workgroups per CU)
+            t.slab = kb < most ? kb : most;
+        } else if (kb > panel_fit(bm)) continue;
+        best = t;
+        if ((rows + bm - 1) / bm * ((n + cols - 1) / cols) >= cus) break;
+    }
+    return best;
 }
 
 constexpr int MAX_K = 131071;          // 128 * 128 * k < 2^31
 long round_up(long v, long m) { return (v + m - 1) / m * m; }
 int es_of(int dt) { return dt == Y3_F32 ? 4 : dt == Y3_BF16 ? 2 : 1; }
+
+// Float rows go through the panel kernel at once where its LDS holds all of k for as many rows as it takes best; otherwise
+// 8-bit rows are made in the workspace first.
+bool fused(const y3_linear_i8_desc *d) {
+    const int bm = d->rows <= 16 ? 16 : d->rows <= 32 ? 32 : 64;
+    return d->k_pad / 64 <= panel_fit(bm);
+}
 
 int check_desc(const y3_linear_i8_desc *d) {
     Y3_REQUIRE(d, Y3_E_INVALID, "linear_i8: null descriptor");
@@ -321,7 +581,7 @@ extern "C" int y3_linear_i8_workspace_bytes(const y3_linear_i8_desc *d, int64_t 
     const int rc = check_desc(d);
     if (rc) return rc;
     Y3_REQUIRE(bytes, Y3_E_INVALID, "linear_i8: null pointer");
-    *bytes = d->dtype == Y3_I8 ? 0 : round_up(d->rows * d->k_pad, 256) + round_up(d->rows * 4, 256);
+    *bytes = d->dtype == Y3_I8 || fused(d) ? 0 : round_up(d->rows * d->k_pad, 256) + round_up(d->rows * 4, 256);
     return Y3_OK;
 }
 
@@ -345,19 +605,20 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     const hipStream_t st = (hipStream_t)stream;
     LinArgs a;
     a.x = (const char *)x; a.x_scale = x_scale; a.x_ld = d->x_ld; a.k16 = (int)round_up(d->k, 16);
-    if (d->dtype != Y3_I8) {
+    if (need) {
         float *s = (float *)((char *)workspace + round_up(d->rows * d->k_pad, 256));
         launch_quant<256>(d->dtype, x, d->rows, d->k, d->x_ld, workspace, d->k_pad, d->k_pad, s, st);
         rc = y3_check_launch("linear_i8 (rows)");
         if (rc) return rc;
         a.x = (const char *)workspace; a.x_scale = s; a.x_ld = d->k_pad; a.k16 = d->k_pad;
     }
+    const long cus = y3_device_cus();
     a.w = (const char *)w; a.w_scale = w_scale; a.bias = bias; a.out = (char *)out;
-    a.rows = d->rows; a.out_ld = d->out_ld; a.n = d->n; a.kb = d->k_pad / 64; a.leaky = d->flags & Y3_CONV_LEAKY;
-    a.n_blocks = (d->n + 63) / 64;
-    const long grid = (d->rows + 63) / 64 * a.n_blocks;
-    Y3_REQUIRE(grid < (1 << 24), Y3_E_INVALID, "linear_i8: grid of %ld workgroups", grid);
-    if (d->out_dtype == Y3_BF16) hipLaunchKernelGGL(linear_i8_kernel<Y3_BF16>, dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(linear_i8_kernel<Y3_F32>, dim3((unsigned)grid), dim3(256), 0, st, a);
-    return y3_check_launch("linear_i8");
+    a.rows = d->rows; a.out_ld = d->out_ld; a.n = d->n; a.k = d->k; a.kb = d->k_pad / 64;
+    a.leaky = d->flags & Y3_CONV_LEAKY; a.out_f32 = d->out_dtype == Y3_F32;
+    if (d->dtype != Y3_I8 && need == 0) {
+        const Panel c = panel_of(d->rows, d->n, a.kb, false, cus);
+        return d->dtype == Y3_BF16 ? launch_panel<Y3_BF16>(a, c, st) : launch_panel<Y3_F32>(a, c, st);
+    }
+    return launch_panel<Y3_I8>(a, panel_of(d->rows, d->n, a.kb, true, cus), st);
 }
