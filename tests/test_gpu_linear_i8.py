@@ -30,8 +30,8 @@ def rule(x):
 
 
 def want(q, s, w, t, b, leaky):
-    """64-bit result and the magnitude that its roundings refer to."""
-    p = (q @ w.T).astype(np.float64) * t.astype(np.float64)[None] * s.astype(np.float64)[:, None]
+    """64-bit result (the sums are whole numbers below 2^53: exact) and the magnitude that its roundings refer to."""
+    p = (q.astype(np.float64) @ w.T.astype(np.float64)) * t.astype(np.float64)[None] * s.astype(np.float64)[:, None]
     y = p + (b.astype(np.float64)[None] if b is not None else 0.0)
     return (np.where(y > 0, y, 0.1 * y) if leaky else y), np.abs(p) + np.abs(y)
 
@@ -115,6 +115,24 @@ def test_product(rows, k, n, x, out):
         q, s = rule(xs.float().numpy())
         got = lay(xs.cuda())
     assert got.dtype == DT[out] and got.shape == (rows, n)
+    close(got, *want(q, s, w, t, b, leaky), out)
+
+
+@pytest.mark.parametrize("rows,k,n", [(4100, 640, 2100), (3000, 512, 3001), (8200, 1037, 1025), (2300, 4096, 4100)])
+@pytest.mark.parametrize("x,out", [("bf16", "bf16"), ("i8", "f32"), ("i8", "bf16"), ("f32", "f32")])
+def test_product_of_many_rows_and_channels(rows, k, n, x, out):
+    """Enough 256 x 256 tiles to fill the card; odd numbers of k-steps, ragged last tiles, more tiles than CUs."""
+    rng = np.random.default_rng(rows + n)
+    bias, leaky = n % 2 == 1, k % 2 == 0
+    lay, w, t, b = layer_of(rng, n, k, bias, leaky, out)
+    if x == "i8":
+        q = rng.integers(-128, 128, (rows, k))
+        s = np.exp(rng.normal(size=rows)).astype(np.float32)
+        got = lay(torch.from_numpy(q.astype(np.int8)).cuda(), scale=torch.from_numpy(s).cuda())
+    else:
+        xs = torch.from_numpy(rows_of(rng, rows, k)).to(DT[x])
+        q, s = rule(xs.float().numpy())
+        got = lay(xs.cuda())
     close(got, *want(q, s, w, t, b, leaky), out)
 
 

@@ -2,7 +2,7 @@
 """Build-time guard (yolo_amd/csrc/Makefile): fail when a kernel that gates LDS reads on hand-counted
 `s_waitcnt vmcnt(N)` has scratch or spills.
 
-conv3x3_c32, conv3x3s2_c64, conv1x1_regw, resblock64 / resblock128 and the ping-pong implicit GEMM count their own
+conv3x3_c32, conv3x3s2_c64, conv1x1_regw, resblock64 / resblock128, the ping-pong implicit GEMM and the 8-bit tile kernel count their own
 stores / LDS-DMA requests in the tile loop and wait with vmcnt(N), N > 0.  (resblock_kernel<256> and the stem drain with
 vmcnt(0) or leave the count to the compiler: a spill there costs time, not correctness.)  That is only correct while the compiler emits no
 other vector-memory instruction there: one scratch spill (buffer_store / buffer_load count in vmcnt) after a compiler or
@@ -12,7 +12,7 @@ import re
 import sys
 
 GUARDED = ("conv3x3_c32_kernel", "conv3x3s2_c64_kernel", "conv1x1_regw_kernel", "resblock64_kernel", "resblock128_kernel",
-           "conv_pp_kernel", "conv_pp_split_kernel")
+           "conv_pp_kernel", "conv_pp_split_kernel", "linear_i8_tile_kernel")
 
 
 def main(path):

@@ -10,19 +10,11 @@
 //
 // Packed weights: MFMA fragments, [n_pad / 16][k_pad / 64][64 lanes][16 bytes]; lane l of a fragment holds channel l & 15,
 // inputs 16 (l >> 4) .. + 15 of the 64.  A wave's fragment load is one contiguous KB whatever n and k are.
-#include "common.h"
-
-typedef __attribute__((ext_vector_type(4))) int i32x4;
+#include "linear_i8.h"
 
 namespace {
 
 constexpr float QTINY = 127.0f * 1.17549435082228750797e-38f;        // 127 * 2^-126: the scale of any row is a normal number
-
-// 16 / 8 bytes at any element's alignment: global memory takes unaligned vector accesses
-typedef u32x4 __attribute__((aligned(2))) u32x4_u2;
-typedef u32x4 __attribute__((aligned(4))) u32x4_u4;
-typedef f32x4 __attribute__((aligned(4))) f32x4_u4;
-typedef unsigned long long __attribute__((aligned(2))) u64_u2;
 
 // ---- eight consecutive elements of a row as fp32 bit patterns ------------------------------------------------------
 template <int DT> struct Chunk;
@@ -212,42 +204,6 @@ __global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld,
 }
 
 // ---- the product ------------------------------------------------------------------------------------------------
-struct LinArgs {
-    const char *x;                     // 8-bit rows on 16 bytes, or float rows
-    const float *x_scale;              // with 8-bit rows
-    const char *w;
-    const float *w_scale, *bias;       // bias may be null
-    char *out;
-    long rows, x_ld, out_ld;
-    int k, k16, n, kb;                 // k rounded up to 16 (bytes of an 8-bit row that may be read), channels, 64-deep k-blocks
-    int leaky, out_f32;
-    int n_groups, wk, slab;            // panel kernel: workgroups along n, waves along k, k-blocks of a slab
-    FastDiv fd_items;
-};
-
-// four channels of one row: scaled, activated, stored.  t, b: the channels' scales and biases.
-__device__ __forceinline__ void store4(const LinArgs &p, long row, int nl, const i32x4 &acc, float s, const f32x4 &t, const f32x4 &b) {
-    if (row >= p.rows || nl >= p.n) return;
-    const bool full = nl + 4 <= p.n;
-    float y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        y[j] = fmaf((float)acc[j] * t[j], s, b[j]);
-        if (p.leaky) y[j] = y[j] > 0.0f ? y[j] : 0.1f * y[j];          // (NaN: the product keeps it)
-    }
-    if (p.out_f32) {
-        float *o = (float *)p.out + row * p.out_ld + nl;
-        if (full) *(f32x4_u4 *)o = f32x4{y[0], y[1], y[2], y[3]};
-        else
-            for (int j = 0; j < p.n - nl; ++j) o[j] = y[j];
-    } else {
-        unsigned short *o = (unsigned short *)p.out + row * p.out_ld + nl;
-        if (full) *(u64_u2 *)o = (unsigned long long)pack_bf16x2(y[2], y[3]) << 32 | pack_bf16x2(y[0], y[1]);
-        else
-            for (int j = 0; j < p.n - nl; ++j) o[j] = f32_to_bf16(y[j]);
-    }
-}
-
 // Panel kernel: a workgroup of eight waves takes 16 RT rows and 16 NT WN channels (WN WK = 8: WN waves side by side along the
 // channels, WK along k).  The rows' 8-bit values are in LDS -- quantised there from float rows, all of k at once, or copied
 // from 8-bit rows in slabs of k -- and every wave reads its weights as whole fragments straight into registers, two
@@ -620,5 +576,6 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
         const Panel c = panel_of(d->rows, d->n, a.kb, false, cus);
         return d->dtype == Y3_BF16 ? launch_panel<Y3_BF16>(a, c, st) : launch_panel<Y3_F32>(a, c, st);
     }
+    if (y3_linear_i8_tile_ok(a, cus)) return y3_linear_i8_tile_launch(a, cus, st);
     return launch_panel<Y3_I8>(a, panel_of(d->rows, d->n, a.kb, true, cus), st);
 }
