@@ -18,8 +18,9 @@ struct LinArgs {
     char *out;
     long rows, x_ld, out_ld;
     int k, k16, n, kb;                 // k rounded up to 16 (bytes of an 8-bit row that may be read), channels, 64-deep k-blocks
-    int leaky, out_f32;
-    int n_groups, wk, slab;            // panel kernel: workgroups along n, waves along k, k-blocks of a slab
+    float slope;                       // of the leaky-ReLU; 1: none
+    int out_f32;
+    int n_groups, slab;                // panel kernel: workgroups along n, k-blocks of a slab
     FastDiv fd_items;
 };
 
@@ -32,8 +33,7 @@ __device__ __forceinline__ void store4(const LinArgs &p, long row, int nl, const
     float y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        y[j] = fmaf((float)acc[j] * t[j], s, b[j]);
-        if (p.leaky) y[j] = y[j] > 0.0f ? y[j] : 0.1f * y[j];          // (NaN: the product keeps it)
+        y[j] = leaky_max(fmaf((float)acc[j] * t[j], s, b[j]), p.slope);
     }
     if (p.out_f32) {
         float *o = (float *)p.out + row * p.out_ld + nl;

@@ -11,6 +11,7 @@
 // Packed weights: MFMA fragments, [n_pad / 16][k_pad / 64][64 lanes][16 bytes]; lane l of a fragment holds channel l & 15,
 // inputs 16 (l >> 4) .. + 15 of the 64.  A wave's fragment load is one contiguous KB whatever n and k are.
 #include "linear_i8.h"
+#include <type_traits>
 
 namespace {
 
@@ -57,6 +58,11 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits);
 __device__ __forceinline__ unsigned q4(unsigned a, unsigned b, unsigned c, unsigned d, float inv);
 
 // ---- the same eight elements as they are stored (registers are what a kernel that keeps many of them is short of) -------
+typedef unsigned short __attribute__((ext_vector_type(2))) u16x2;
+__device__ __forceinline__ unsigned pk_umax16(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
 template <int DT> struct Raw;
 template <> struct Raw<Y3_BF16> {
     static constexpr int N = 4;
@@ -72,9 +78,14 @@ template <> struct Raw<Y3_BF16> {
         }
     }
     static __device__ __forceinline__ unsigned amax(const unsigned (&v)[4]) {      
-        unsigned m = 0;
+        const unsigned m = magnitudes(v);
+        return max(m << 16, m & 0xffff0000u);
+    }
+    // the largest magnitudes of the even and of the odd elements, as bf16 bits in the two halves
+    static __device__ __forceinline__ unsigned magnitudes(const unsigned (&v)[4]) {
+        unsigned m = v[0] & 0x7fff7fffu;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = max(m, max(v[j] << 16 & 0x7fffffffu, v[j] & 0x7fff0000u));
+        for (int j = 1; j < 4; ++j) m = pk_umax16(m, v[j] & 0x7fff7fffu);
         return m;
     }
     static __device__ __forceinline__ unsigned long long quantize(const unsigned (&v)[4], float inv) {
@@ -213,28 +224,110 @@ __global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld,
 constexpr int PN_THREADS = 512, PN_WAVES = 8;
 constexpr int PN_LDS_MAX = 160 * 1024;
 
-template <int XT, int RT, int NT>
+// Maximum over the LPR lanes of a row, in all of them: DPP within 16, then the halves of 32 and 64 side by side.
+template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(unsigned v, F f) {
+    v = f(v, dpp_u<0xB1>(v));
+    v = f(v, dpp_u<0x4E>(v));
+    v = f(v, dpp_u<0x141>(v));
+    v = f(v, dpp_u<0x140>(v));
+    if constexpr (LPR >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = f(s[0], s[1]);
+    }
+    if constexpr (LPR >= 64) {
+        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = f(s[0], s[1]);
+    }
+    return v;
+}
+
+// Float rows -> 8-bit rows in LDS.  A wave takes 64 / LPR rows at a time, LPR lanes each, a lane's CPL chunks of eight values
+// LPR chunks apart, and NB such groups at once: all their loads are in flight together, the maxima of a group are one
+// register, and lane n of every 16 divides for group n.  Rows from nr on repeat the last one.
+template <int XT, int LPR, int CPL>
+__device__ __forceinline__ void quantize_panel(const LinArgs &p, const char *x0, int nr, char *rows_lds, int pitch, float *row_s, int wave, int lane) {
+    constexpr int ES = XT == Y3_BF16 ? 2 : 4, N = Raw<XT>::N, RG = 64 / LPR, NB = 64 / N / CPL < 8 ? 64 / N / CPL : 8;
+    const int l = lane & (LPR - 1), in_group = LPR == 64 ? 0 : lane / LPR;
+    const bool full = p.k == LPR * CPL * 8;
+    for (int b0 = 0; (wave + PN_WAVES * b0) * RG < nr; b0 += NB) {
+        unsigned v[NB][CPL][N], m[NB];
+        const auto row_of = [&](int n) { return min((wave + PN_WAVES * (b0 + n)) * RG + in_group, nr - 1); };
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const char *xr = x0 + row_of(n) * p.x_ld * ES;
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) Raw<XT>::load(xr, (l + c * LPR) * 8, full ? 8 : p.k - (l + c * LPR) * 8, v[n][c]);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            if constexpr (XT == Y3_BF16) {
+                m[n] = Raw<XT>::magnitudes(v[n][0]);
+#pragma unroll
+                for (int c = 1; c < CPL; ++c) m[n] = pk_umax16(m[n], Raw<XT>::magnitudes(v[n][c]));
+                m[n] = max(m[n] >> 16, m[n] & 0xffffu);
+            } else {
+                m[n] = Raw<XT>::amax(v[n][0]);
+#pragma unroll
+                for (int c = 1; c < CPL; ++c) m[n] = max(m[n], Raw<XT>::amax(v[n][c]));
+            }
+        }
+        if constexpr (XT == Y3_BF16 && NB % 2 == 0) {            // two groups' 16-bit maxima in one register
+#pragma unroll
+            for (int n = 0; n < NB; n += 2) {
+                const unsigned both = lanes_max<LPR>(m[n] | m[n + 1] << 16, [](unsigned a, unsigned b) { return pk_umax16(a, b); });
+                m[n] = both << 16;
+                m[n + 1] = both & 0xffff0000u;
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) m[n] = lanes_max<LPR>(XT == Y3_BF16 ? m[n] << 16 : m[n], [](unsigned a, unsigned b) { return max(a, b); });
+        }
+        unsigned mine = m[0];
+        int row = row_of(0);
+#pragma unroll
+        for (int n = 1; n < NB; ++n)
+            if ((lane & 15) == n) { mine = m[n]; row = row_of(n); }
+        const RowScale r = row_scale(mine);
+        if (l < NB) row_s[row] = r.s;
+        const unsigned inv_bits = __float_as_uint(r.finite ? r.inv : 0.0f);
+        const auto write = [&](auto NN) {
+            constexpr int n = decltype(NN)::value;
+            if constexpr (n < NB) {
+                const float inv = __uint_as_float(dpp_u<0x150 + n>(inv_bits));
+                char *to = rows_lds + row_of(n) * pitch + l * 8;
+#pragma unroll
+                for (int c = 0; c < CPL; ++c)
+                    if (full || (l + c * LPR) * 8 < p.kb * 64) *(unsigned long long *)(to + c * LPR * 8) = Raw<XT>::quantize(v[n][c], inv);
+            }
+        };
+        write(std::integral_constant<int, 0>{}); write(std::integral_constant<int, 1>{}); write(std::integral_constant<int, 2>{});
+        write(std::integral_constant<int, 3>{}); write(std::integral_constant<int, 4>{}); write(std::integral_constant<int, 5>{});
+        write(std::integral_constant<int, 6>{}); write(std::integral_constant<int, 7>{});
+    }
+}
+
+template <int XT, int RT, int NT, int WK>
 __global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(4)))
 void linear_i8_panel_kernel(const LinArgs p) {
-    constexpr int BM = 16 * RT, U = NT == 1 ? 4 : NT == 2 ? 2 : 1;       // U: k-blocks of a group of weight fragments
+    constexpr int BM = 16 * RT, wn_count = PN_WAVES / WK, cols = 16 * NT * wn_count;         // rows, channels of the workgroup
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int frow = lane & 15, fq = lane >> 4;
-    const int wn_count = PN_WAVES / p.wk, wn = wave % wn_count, wk = wave / wn_count;
+    const int wn = wave % wn_count, wk = wave / wn_count;
     const int pitch = p.slab * 64 + 32;
-    const int cols = 16 * NT * wn_count;                         // channels of the workgroup
     const long m0 = (long)(blockIdx.x / p.n_groups) * BM;
     const int n0 = (int)(blockIdx.x % p.n_groups) * cols;
     const int nr = (int)(p.rows - m0 < BM ? p.rows - m0 : BM);   // rows that are there
-    const int area = max(BM * pitch, p.wk > 1 ? PN_WAVES * RT * NT * 1024 : 0);
+    const int area = max(BM * pitch, WK > 1 ? PN_WAVES * RT * NT * 1024 : 0);
     float *row_s = (float *)(smem + area), *row_inv = row_s + BM, *col_t = row_inv + BM, *col_b = col_t + cols;
     unsigned *row_max = (unsigned *)row_inv;
 
     const int frags = (p.n + 15) >> 4;
-    const char *wp[NT];                                          // this wave's fragments (past the last channel: the last one's)
+    // this wave's fragments (past the last channel: the last one's), as offsets from the workgroup's first: below 64 MB
+    const auto rs_w = __builtin_amdgcn_make_buffer_rsrc((void *)(p.w + (long)(n0 >> 4) * p.kb * 1024), 0, 0x7fffffff, 0x00020000);
+    unsigned w_off[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) wp[i] = p.w + (long)min((n0 >> 4) + wn * NT + i, frags - 1) * p.kb * 1024;
-    const unsigned w_lane = lane * 16;
+    for (int i = 0; i < NT; ++i) w_off[i] = (unsigned)min(wn * NT + i, frags - 1 - (n0 >> 4)) * (unsigned)p.kb * 1024u;
 
     for (int c = tid; c < cols; c += PN_THREADS) {
         const int ch = min(n0 + c, p.n - 1);
@@ -244,116 +337,138 @@ void linear_i8_panel_kernel(const LinArgs p) {
     if constexpr (XT == Y3_I8) {
         if (tid < BM) row_s[tid] = p.x_scale[min(m0 + tid, p.rows - 1)];
     } else {
-        // float rows -> 8-bit rows: chunks of eight values; sixteen neighbouring lanes always share a row
-        constexpr int NI = XT == Y3_BF16 ? 16 : 8;               // chunks a thread keeps between the two looks at them
-        const int per_row = p.kb * 8, items = nr * per_row;
         const char *x0 = p.x + m0 * p.x_ld * (XT == Y3_BF16 ? 2 : 4);
-        if (tid < BM) row_max[tid] = 0;
-        __syncthreads();
-        const auto at = [&](int item, int &row, int &k0) {
-            row = fast_div(item, p.fd_items);
-            k0 = (item - row * per_row) * 8;
-        };
-        const auto fetch = [&](int item, unsigned (&v)[Raw<XT>::N]) {
-            int row, k0;
-            at(item, row, k0);
-            Raw<XT>::load(x0 + row * p.x_ld * (XT == Y3_BF16 ? 2 : 4), k0, p.k - k0, v);
-        };
-        const auto look = [&](int item, const unsigned (&v)[Raw<XT>::N]) {
-            int row, k0;
-            at(item, row, k0);
-            unsigned m = Raw<XT>::amax(v);
-            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));
-            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));
-            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));
-            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xf, 0xf, false));
-            if (frow == 0) atomicMax(&row_max[row], m);
-        };
-        const auto write = [&](int item, const unsigned (&v)[Raw<XT>::N]) {
-            int row, k0;
-            at(item, row, k0);
-            const float inv = row_inv[row];
-            *(unsigned long long *)(smem + row * pitch + k0) = inv > 0.0f ? Raw<XT>::quantize(v, inv) : 0;
-        };
-        const bool keep = items <= NI * PN_THREADS;
-        unsigned v[NI][Raw<XT>::N];
-        for (int g = 0; g < items; g += NI * PN_THREADS) {
+        const int chunks = p.kb * 8;
+        if (RT == 1 && (nr < PN_WAVES || chunks > 512)) {
+            // few or long rows: all waves on the chunks of all of them, sixteen neighbouring lanes always in one row
+            constexpr int NI = 4;                                // chunks a thread keeps between the two looks at them
+            const int items = nr * chunks;
+            if (tid < BM) row_max[tid] = 0;
+            __syncthreads();
+            const auto at = [&](int item, int &row, int &k0) {
+                row = fast_div(item, p.fd_items);
+                k0 = (item - row * chunks) * 8;
+            };
+            unsigned v[NI][Raw<XT>::N];
+            const auto fetch = [&](int g) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                if (g + i * PN_THREADS + tid < items) fetch(g + i * PN_THREADS + tid, v[i]);
+                for (int i = 0; i < NI; ++i) {
+                    int row, k0;
+                    at(min(g + i * PN_THREADS + tid, items - 1), row, k0);
+                    Raw<XT>::load(x0 + row * p.x_ld * (XT == Y3_BF16 ? 2 : 4), k0, p.k - k0, v[i]);
+                }
+            };
+            for (int g = 0; g < items; g += NI * PN_THREADS) {
+                fetch(g);
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                if (g + i * PN_THREADS + tid < items) look(g + i * PN_THREADS + tid, v[i]);
-        }
-        __syncthreads();
-        if (tid < BM) {
-            const RowScale r = row_scale(row_max[tid]);
-            row_s[tid] = r.s;
-            row_inv[tid] = r.finite ? r.inv : -1.0f;
-        }
-        __syncthreads();
-        for (int g = 0; g < items; g += NI * PN_THREADS) {
-            if (!keep) {
-#pragma unroll
-                for (int i = 0; i < NI; ++i)
-                    if (g + i * PN_THREADS + tid < items) fetch(g + i * PN_THREADS + tid, v[i]);
+                for (int i = 0; i < NI; ++i) {
+                    int row, k0;
+                    at(min(g + i * PN_THREADS + tid, items - 1), row, k0);
+                    const unsigned m = lanes_max<16>(Raw<XT>::amax(v[i]), [](unsigned a, unsigned b) { return max(a, b); });
+                    if (frow == 0 && g + i * PN_THREADS + tid < items) atomicMax(&row_max[row], m);
+                }
             }
+            __syncthreads();
+            if (tid < BM) {
+                const RowScale r = row_scale(row_max[tid]);
+                row_s[tid] = r.s;
+                row_inv[tid] = r.finite ? r.inv : 0.0f;
+            }
+            __syncthreads();
+            for (int g = 0; g < items; g += NI * PN_THREADS) {
+                if (items > NI * PN_THREADS) fetch(g);
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                if (g + i * PN_THREADS + tid < items) write(g + i * PN_THREADS + tid, v[i]);
-        }
+                for (int i = 0; i < NI; ++i) {
+                    if (g + i * PN_THREADS + tid >= items) break;
+                    int row, k0;
+                    at(g + i * PN_THREADS + tid, row, k0);
+                    *(unsigned long long *)(smem + row * pitch + k0) = Raw<XT>::quantize(v[i], row_inv[row]);
+                }
+            }
+        } else if (chunks <= 16) quantize_panel<XT, 16, 1>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 32) quantize_panel<XT, 32, 1>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 64) quantize_panel<XT, 64, 1>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 128) quantize_panel<XT, 64, 2>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 256) quantize_panel<XT, 64, 4>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else quantize_panel<XT, 64, 8>(p, x0, nr, smem, pitch, row_s, wave, lane);
     }
 
     i32x4 acc[RT][NT] = {};
-    const char *xl[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) xl[r] = smem + min(r * 16 + frow, nr - 1) * pitch + fq * 16;
+    const auto weight = [&](int i, int kb) {
+        return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_w, lane * 16, w_off[i] + (unsigned)kb * 1024u, 0));
+    };
     for (int s0 = 0; s0 < p.kb; s0 += p.slab) {
-        const int s_kb = min(p.slab, p.kb - s0);                 // k-blocks of this slab
-        // this wave's: wk, wk + WK, ...
-        const int mine = s_kb > wk ? (s_kb - wk + p.wk - 1) / p.wk : 0;
-        i32x4 wf[2][U][NT];
-        const auto weights = [&](int g, i32x4 (&f)[U][NT]) {     // group g (past the end: any fragment, not multiplied)
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const long kb = min(s0 + wk + (g * U + u) * p.wk, p.kb - 1);
-#pragma unroll
-                for (int i = 0; i < NT; ++i) f[u][i] = *(const i32x4 *)(wp[i] + kb * 1024 + w_lane);
+        const int s_kb = min(p.slab, p.kb - s0);                 // k-blocks of this slab: an even number
+        const auto slab = [&]() {
+            if constexpr (XT == Y3_I8) {
+                if (s0) __syncthreads();                         // (the previous slab has been read)
+                const int chunks = s_kb * 4;                     // 16 bytes each
+                for (int i = tid; i < nr * chunks; i += PN_THREADS) {
+                    const int row = i / chunks, c = i - row * chunks, k0 = s0 * 64 + c * 16;
+                    u32x4 v = {0, 0, 0, 0};
+                    if (k0 < p.k16) v = *(const u32x4 *)(p.x + (m0 + row) * p.x_ld + k0);
+                    *(u32x4 *)(smem + row * pitch + c * 16) = v;
+                }
             }
+            __syncthreads();
         };
-        weights(0, wf[0]);
-        if constexpr (XT == Y3_I8) {
-            if (s0) __syncthreads();                             // (the previous slab has been read)
-            const int chunks = s_kb * 4;                         // 16 bytes each
-            for (int i = tid; i < nr * chunks; i += PN_THREADS) {
-                const int row = i / chunks, c = i - row * chunks, k0 = s0 * 64 + c * 16;
-                u32x4 v = {0, 0, 0, 0};
-                if (k0 < p.k16) v = *(const u32x4 *)(p.x + (m0 + row) * p.x_ld + k0);
-                *(u32x4 *)(smem + row * pitch + c * 16) = v;
+        const char *xl[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) xl[r] = smem + min(r * 16 + frow, nr - 1) * pitch + fq * 16;
+        if constexpr (WK == 1) {                                 // two k-blocks' weights in turn: one multiplied, one on its way
+            i32x4 wa[NT], wb[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wa[i] = weight(i, s0);
+            slab();
+            const auto multiply = [&](const i32x4 (&f)[NT], int at) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const i32x4 xf = *(const i32x4 *)(xl[r] + at);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) acc[r][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i], xf, acc[r][i], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            for (int kb = 0; kb < s_kb; kb += 2) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) wb[i] = weight(i, s0 + kb + 1);
+                multiply(wa, 0);
+                const int next = min(s0 + kb + 2, p.kb - 1);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) wa[i] = weight(i, next);
+                multiply(wb, 64);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) xl[r] += 128;
             }
-        }
-        __syncthreads();
-        const auto multiply = [&](int g, const i32x4 (&f)[U][NT]) {
+        } else {                                                 // this wave's k-blocks: wk, wk + WK, ..., in groups of U
+            static_assert(NT == 1, "waves along k have one block of channels");
+            constexpr int U = 4;
+            const int mine = s_kb > wk ? (s_kb - wk + WK - 1) / WK : 0;
+            i32x4 wf[2][U];
+            const auto weights = [&](int g, i32x4 (&f)[U]) {     // (past the end: any fragment, not multiplied)
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (g * U + u >= mine) break;
-                const int kb = wk + (g * U + u) * p.wk;
-                i32x4 xf[RT];
+                for (int u = 0; u < U; ++u) f[u] = weight(0, min(s0 + wk + (g * U + u) * WK, p.kb - 1));
+            };
+            weights(0, wf[0]);
+            slab();
+            const auto multiply = [&](int g, const i32x4 (&f)[U]) {
 #pragma unroll
-                for (int r = 0; r < RT; ++r) xf[r] = *(const i32x4 *)(xl[r] + kb * 64);
+                for (int u = 0; u < U; ++u) {
+                    if (g * U + u >= mine) break;
+                    const int kb = wk + (g * U + u) * WK;
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) acc[r][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[u][i], xf[r], acc[r][i], 0, 0, 0);
-            }
-        };
-        const int groups = (mine + U - 1) / U;
-        for (int g = 0; g < groups; g += 2) {
-            if (g + 1 < groups) weights(g + 1, wf[1]);
-            multiply(g, wf[0]);
-            if (g + 1 < groups) {
-                if (g + 2 < groups) weights(g + 2, wf[0]);
-                multiply(g + 1, wf[1]);
+                    for (int r = 0; r < RT; ++r) acc[r][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[u], *(const i32x4 *)(xl[r] + kb * 64), acc[r][0], 0, 0, 0);
+                }
+            };
+            const int groups = (mine + U - 1) / U;
+            for (int g = 0; g < groups; g += 2) {
+                if (g + 1 < groups) weights(g + 1, wf[1]);
+                multiply(g, wf[0]);
+                if (g + 1 < groups) {
+                    if (g + 2 < groups) weights(g + 2, wf[0]);
+                    multiply(g + 1, wf[1]);
+                }
             }
         }
     }
@@ -361,7 +476,38 @@ void linear_i8_panel_kernel(const LinArgs p) {
     const auto put = [&](int r, int c, const i32x4 &v) {         // 16 x 16 block: rows r .. r + 15, channels c .. c + 15 of the workgroup's
         store4(p, m0 + r + frow, n0 + c + fq * 4, v, row_s[r + frow], *(const f32x4 *)(col_t + c + fq * 4), *(const f32x4 *)(col_b + c + fq * 4));
     };
-    if (p.wk == 1) {
+    if (WK == 1 && nr == BM && n0 + cols <= p.n) {             // (the same in all waves) nothing to look at on the way out
+        f32x4 t[NT], b[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            t[i] = *(const f32x4 *)(col_t + (wn * NT + i) * 16 + fq * 4);
+            b[i] = *(const f32x4 *)(col_b + (wn * NT + i) * 16 + fq * 4);
+        }
+        const long first = (m0 + frow) * p.out_ld + n0 + wn * NT * 16;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const float s = row_s[r * 16 + frow];
+            f32x4 y[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[i][j] = leaky_max(fmaf((float)acc[r][i][j] * t[i][j], s, b[i][j]), p.slope);
+            const long at = first + r * 16 * p.out_ld;
+            if (p.out_f32) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) *(f32x4_u4 *)((float *)p.out + at + i * 16 + fq * 4) = y[i];
+            } else if constexpr (NT == 1) {
+                *(u64_u2 *)((unsigned short *)p.out + at + fq * 4) = (unsigned long long)pack_bf16x2(y[0][2], y[0][3]) << 32 | pack_bf16x2(y[0][0], y[0][1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT; i += 2) {                // two blocks change places between quarter-waves: eight channels per lane
+                    const auto s0 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(y[i][0], y[i][1]), pack_bf16x2(y[i + 1][0], y[i + 1][1]), false, false);
+                    const auto s1 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(y[i][2], y[i][3]), pack_bf16x2(y[i + 1][2], y[i + 1][3]), false, false);
+                    *(u32x4_u2 *)((unsigned short *)p.out + at + i * 16 + ((fq & 1) ? 16 + (fq - 1) * 4 : fq * 4)) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                }
+            }
+        }
+    } else if (WK == 1) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -377,7 +523,7 @@ void linear_i8_panel_kernel(const LinArgs p) {
         for (int b = wave; b < wn_count * RT * NT; b += PN_WAVES) {          // block b = (wn, r, i)
             const int bw = b / (RT * NT), ri = b % (RT * NT);
             i32x4 v = sums[(bw * RT * NT + ri) * 64 + lane];
-            for (int k = 1; k < p.wk; ++k) v += sums[((k * wn_count + bw) * RT * NT + ri) * 64 + lane];
+            for (int k = 1; k < WK; ++k) v += sums[((k * wn_count + bw) * RT * NT + ri) * 64 + lane];
             put(ri / NT * 16, (bw * NT + ri % NT) * 16, v);
         }
     }
@@ -389,38 +535,40 @@ int panel_area(int rt, int nt, int wk, int slab) {
 }
 int panel_lds(int rt, int nt, int wk, int slab) { return panel_area(rt, nt, wk, slab) + (2 * 16 * rt + 2 * 16 * nt * (PN_WAVES / wk)) * 4; }
 
-template <int XT, int RT, int NT>
+template <int XT, int RT, int NT, int WK>
 int launch_panel_as(LinArgs a, hipStream_t st) {
     static thread_local int attr_dev = -1;
     int dev = 0;
     (void)hipGetDevice(&dev);
     if (attr_dev != dev) {
-        if (hipFuncSetAttribute((const void *)linear_i8_panel_kernel<XT, RT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, PN_LDS_MAX) != hipSuccess) {
+        if (hipFuncSetAttribute((const void *)linear_i8_panel_kernel<XT, RT, NT, WK>, hipFuncAttributeMaxDynamicSharedMemorySize, PN_LDS_MAX) != hipSuccess) {
             y3_set_error("linear_i8: cannot reserve %d bytes of LDS", PN_LDS_MAX);
             return Y3_E_LAUNCH;
         }
         attr_dev = dev;
     }
-    const int cols = 16 * NT * (PN_WAVES / a.wk);
+    constexpr int cols = 16 * NT * (PN_WAVES / WK);
     a.n_groups = (a.n + cols - 1) / cols;
     const long grid = (a.rows + 16 * RT - 1) / (16 * RT) * a.n_groups;
     Y3_REQUIRE(grid < (1 << 23), Y3_E_INVALID, "linear_i8: grid of %ld workgroups", grid);
-    hipLaunchKernelGGL((linear_i8_panel_kernel<XT, RT, NT>), dim3((unsigned)grid), dim3(PN_THREADS), panel_lds(RT, NT, a.wk, a.slab), st, a);
+    hipLaunchKernelGGL((linear_i8_panel_kernel<XT, RT, NT, WK>), dim3((unsigned)grid), dim3(PN_THREADS), panel_lds(RT, NT, WK, a.slab), st, a);
     return y3_check_launch("linear_i8");
 }
 
 struct Panel { int rt, nt, wk, slab; };
-int panel_fit(int bm) { return (PN_LDS_MAX - 6 * 1024) / bm / 64 - 1; }       // k-blocks of bm rows that LDS holds
+int panel_fit(int bm) {                // k-blocks of bm rows that LDS holds, and quantize_panel takes (RT > 1: up to 4096)
+    const int fit = (PN_LDS_MAX - 6 * 1024) / bm / 64 - 1;
+    return bm > 16 && fit > 64 ? 64 : fit;
+}
 template <int XT> int launch_panel(const LinArgs &a, const Panel &c, hipStream_t st) {
     LinArgs b = a;
-    b.wk = c.wk;
     b.slab = c.slab;
     b.fd_items = make_fastdiv(a.kb * 8);
-    if (c.rt == 1) return launch_panel_as<XT, 1, 1>(b, st);
-    if (c.rt == 2) return launch_panel_as<XT, 2, 1>(b, st);
-    if (c.nt == 1) return launch_panel_as<XT, 4, 1>(b, st);
-    if (c.nt == 2) return launch_panel_as<XT, 4, 2>(b, st);
-    return launch_panel_as<XT, 4, 4>(b, st);
+    if (c.rt == 1) return c.wk == 2 ? launch_panel_as<XT, 1, 1, 2>(b, st) : c.wk == 4 ? launch_panel_as<XT, 1, 1, 4>(b, st) : launch_panel_as<XT, 1, 1, 8>(b, st);
+    if (c.rt == 2) return c.wk == 1 ? launch_panel_as<XT, 2, 1, 1>(b, st) : launch_panel_as<XT, 2, 1, 2>(b, st);
+    if (c.nt == 1) return launch_panel_as<XT, 4, 1, 1>(b, st);
+    if (c.nt == 2) return launch_panel_as<XT, 4, 2, 1>(b, st);
+    return launch_panel_as<XT, 4, 4, 1>(b, st);
 }
 
 // The largest block of rows and channels that still gives every CU a workgroup (weights are read once per 16 RT rows,
@@ -571,7 +719,7 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     const long cus = y3_device_cus();
     a.w = (const char *)w; a.w_scale = w_scale; a.bias = bias; a.out = (char *)out;
     a.rows = d->rows; a.out_ld = d->out_ld; a.n = d->n; a.k = d->k; a.kb = d->k_pad / 64;
-    a.leaky = d->flags & Y3_CONV_LEAKY; a.out_f32 = d->out_dtype == Y3_F32;
+    a.slope = d->flags & Y3_CONV_LEAKY ? 0.1f : 1.0f; a.out_f32 = d->out_dtype == Y3_F32;
     if (d->dtype != Y3_I8 && need == 0) {
         const Panel c = panel_of(d->rows, d->n, a.kb, false, cus);
         return d->dtype == Y3_BF16 ? launch_panel<Y3_BF16>(a, c, st) : launch_panel<Y3_F32>(a, c, st);

@@ -237,8 +237,7 @@ void linear_i8_tile_kernel(const LinArgs p, int m_tiles, int n_tiles, int total)
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            y[i][j] = fmaf((float)acc[2 * pr + i][mi][j] * t[i][j], s[mi], b[i][j]);
-                            if (p.leaky) y[i][j] = y[i][j] > 0.0f ? y[i][j] : 0.1f * y[i][j];
+                            y[i][j] = leaky_max(fmaf((float)acc[2 * pr + i][mi][j] * t[i][j], s[mi], b[i][j]), p.slope);
                         }
                     // the two 16-channel blocks change places between neighbouring quarter-waves: eight channels per lane
                     const auto s0 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(y[0][0], y[0][1]), pack_bf16x2(y[1][0], y[1][1]), false, false);
