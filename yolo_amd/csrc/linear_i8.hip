@@ -66,8 +66,8 @@ __device__ __forceinline__ unsigned pk_umax16(unsigned a, unsigned b) {
 template <int DT> struct Raw;
 template <> struct Raw<Y3_BF16> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void load(const char *row, int k0, int left, unsigned (&v)[4]) {
-        const unsigned short *p = (const unsigned short *)row + k0;
+    static __device__ __forceinline__ void load(const char *row, unsigned k0, int left, unsigned (&v)[4]) {
+        const unsigned short *p = (const unsigned short *)(row + k0 * 2);
         if (left >= 8) {
             const u32x4 r = *(const u32x4_u2 *)p;
 #pragma unroll
@@ -96,7 +96,7 @@ template <> struct Raw<Y3_BF16> {
 };
 template <> struct Raw<Y3_F32> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void load(const char *row, int k0, int left, unsigned (&v)[8]) { Chunk<Y3_F32>::load(row, k0, left, v); }
+    static __device__ __forceinline__ void load(const char *row, unsigned k0, int left, unsigned (&v)[8]) { Chunk<Y3_F32>::load(row + k0 * 4, 0, left, v); }
     static __device__ __forceinline__ unsigned amax(const unsigned (&v)[8]) { return amax8(v, 0); }
     static __device__ __forceinline__ unsigned long long quantize(const unsigned (&v)[8], float inv) {
         return (unsigned long long)q4(v[4], v[5], v[6], v[7], inv) << 32 | q4(v[0], v[1], v[2], v[3], inv);
@@ -244,20 +244,30 @@ template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(uns
 // Float rows -> 8-bit rows in LDS.  A wave takes 64 / LPR rows at a time, LPR lanes each, a lane's CPL chunks of eight values
 // LPR chunks apart, and NB such groups at once: all their loads are in flight together, the maxima of a group are one
 // register, and lane n of every 16 divides for group n.  Rows from nr on repeat the last one.
-template <int XT, int LPR, int CPL>
+template <int XT, int BM, int LPR, int CPL, int REGS>
 __device__ __forceinline__ void quantize_panel(const LinArgs &p, const char *x0, int nr, char *rows_lds, int pitch, float *row_s, int wave, int lane) {
-    constexpr int ES = XT == Y3_BF16 ? 2 : 4, N = Raw<XT>::N, RG = 64 / LPR, NB = 64 / N / CPL < 8 ? 64 / N / CPL : 8;
+    constexpr int ES = XT == Y3_BF16 ? 2 : 4, N = Raw<XT>::N, RG = 64 / LPR;
+    constexpr int FIT = REGS / N / CPL < 1 ? 1 : REGS / N / CPL, EACH = (BM / RG + PN_WAVES - 1) / PN_WAVES, NB0 = FIT < EACH ? FIT : EACH;
+    constexpr int NB = NB0 < 8 ? NB0 : 8;
     const int l = lane & (LPR - 1), in_group = LPR == 64 ? 0 : lane / LPR;
-    const bool full = p.k == LPR * CPL * 8;
+    const bool full = p.k == LPR * CPL * 8 && nr == BM;
+    const long ld = p.x_ld * ES, lane_ld = in_group * ld;
+    const int lane_pitch = in_group * pitch + l * 8;
     for (int b0 = 0; (wave + PN_WAVES * b0) * RG < nr; b0 += NB) {
         unsigned v[NB][CPL][N], m[NB];
         const auto row_of = [&](int n) { return min((wave + PN_WAVES * (b0 + n)) * RG + in_group, nr - 1); };
+        // (FULL: every lane's chunks are whole and every group has its rows: nothing to look at)
+        const auto group_of = [&](int n) { return min((wave + PN_WAVES * (b0 + n)) * RG, BM - RG); };
+        const auto load = [&](auto FULL) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const char *xr = x0 + row_of(n) * p.x_ld * ES;
+            for (int n = 0; n < NB; ++n) {
+                const char *xr = decltype(FULL)::value ? x0 + group_of(n) * ld + lane_ld : x0 + row_of(n) * ld;
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) Raw<XT>::load(xr, (l + c * LPR) * 8, full ? 8 : p.k - (l + c * LPR) * 8, v[n][c]);
-        }
+                for (int c = 0; c < CPL; ++c) Raw<XT>::load(xr, (l + c * LPR) * 8, decltype(FULL)::value ? 8 : p.k - (l + c * LPR) * 8, v[n][c]);
+            }
+        };
+        if (full) load(std::true_type{});
+        else load(std::false_type{});
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             if constexpr (XT == Y3_BF16) {
@@ -288,27 +298,33 @@ __device__ __forceinline__ void quantize_panel(const LinArgs &p, const char *x0,
         for (int n = 1; n < NB; ++n)
             if ((lane & 15) == n) { mine = m[n]; row = row_of(n); }
         const RowScale r = row_scale(mine);
-        if (l < NB) row_s[row] = r.s;
+        if (l < NB) row_s[row] = r.s;                            // (NB <= 8 <= LPR)
         const unsigned inv_bits = __float_as_uint(r.finite ? r.inv : 0.0f);
-        const auto write = [&](auto NN) {
+        const auto write = [&](auto NN, auto FULL) {
             constexpr int n = decltype(NN)::value;
             if constexpr (n < NB) {
                 const float inv = __uint_as_float(dpp_u<0x150 + n>(inv_bits));
-                char *to = rows_lds + row_of(n) * pitch + l * 8;
+                char *to = rows_lds + (decltype(FULL)::value ? group_of(n) * pitch + lane_pitch : row_of(n) * pitch + l * 8);
 #pragma unroll
                 for (int c = 0; c < CPL; ++c)
-                    if (full || (l + c * LPR) * 8 < p.kb * 64) *(unsigned long long *)(to + c * LPR * 8) = Raw<XT>::quantize(v[n][c], inv);
+                    if (decltype(FULL)::value || (l + c * LPR) * 8 < p.kb * 64) *(unsigned long long *)(to + c * LPR * 8) = Raw<XT>::quantize(v[n][c], inv);
             }
         };
-        write(std::integral_constant<int, 0>{}); write(std::integral_constant<int, 1>{}); write(std::integral_constant<int, 2>{});
-        write(std::integral_constant<int, 3>{}); write(std::integral_constant<int, 4>{}); write(std::integral_constant<int, 5>{});
-        write(std::integral_constant<int, 6>{}); write(std::integral_constant<int, 7>{});
+        const auto write_all = [&](auto FULL) {
+            write(std::integral_constant<int, 0>{}, FULL); write(std::integral_constant<int, 1>{}, FULL);
+            write(std::integral_constant<int, 2>{}, FULL); write(std::integral_constant<int, 3>{}, FULL);
+            write(std::integral_constant<int, 4>{}, FULL); write(std::integral_constant<int, 5>{}, FULL);
+            write(std::integral_constant<int, 6>{}, FULL); write(std::integral_constant<int, 7>{}, FULL);
+        };
+        if (full) write_all(std::true_type{});
+        else write_all(std::false_type{});
     }
 }
 
 template <int XT, int RT, int NT, int WK>
-__global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(4)))
+__global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(NT == 4 ? 4 : 6)))
 void linear_i8_panel_kernel(const LinArgs p) {
+    constexpr int REGS = NT == 4 ? 64 : 32;                      // of float rows on their way, per lane
     constexpr int BM = 16 * RT, wn_count = PN_WAVES / WK, cols = 16 * NT * wn_count;         // rows, channels of the workgroup
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -385,12 +401,12 @@ void linear_i8_panel_kernel(const LinArgs p) {
                     *(unsigned long long *)(smem + row * pitch + k0) = Raw<XT>::quantize(v[i], row_inv[row]);
                 }
             }
-        } else if (chunks <= 16) quantize_panel<XT, 16, 1>(p, x0, nr, smem, pitch, row_s, wave, lane);
-        else if (chunks <= 32) quantize_panel<XT, 32, 1>(p, x0, nr, smem, pitch, row_s, wave, lane);
-        else if (chunks <= 64) quantize_panel<XT, 64, 1>(p, x0, nr, smem, pitch, row_s, wave, lane);
-        else if (chunks <= 128) quantize_panel<XT, 64, 2>(p, x0, nr, smem, pitch, row_s, wave, lane);
-        else if (chunks <= 256) quantize_panel<XT, 64, 4>(p, x0, nr, smem, pitch, row_s, wave, lane);
-        else quantize_panel<XT, 64, 8>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        } else if (chunks <= 16) quantize_panel<XT, BM, 16, 1, REGS>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 32) quantize_panel<XT, BM, 32, 1, REGS>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 64) quantize_panel<XT, BM, 64, 1, REGS>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 128) quantize_panel<XT, BM, 64, 2, REGS>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else if (chunks <= 256) quantize_panel<XT, BM, 64, 4, REGS>(p, x0, nr, smem, pitch, row_s, wave, lane);
+        else quantize_panel<XT, BM, 64, 8, REGS>(p, x0, nr, smem, pitch, row_s, wave, lane);
     }
 
     i32x4 acc[RT][NT] = {};
@@ -476,7 +492,7 @@ void linear_i8_panel_kernel(const LinArgs p) {
     const auto put = [&](int r, int c, const i32x4 &v) {         // 16 x 16 block: rows r .. r + 15, channels c .. c + 15 of the workgroup's
         store4(p, m0 + r + frow, n0 + c + fq * 4, v, row_s[r + frow], *(const f32x4 *)(col_t + c + fq * 4), *(const f32x4 *)(col_b + c + fq * 4));
     };
-    if (WK == 1 && nr == BM && n0 + cols <= p.n) {             // (the same in all waves) nothing to look at on the way out
+    if (WK == 1 && nr == BM && n0 + (wn + 1) * 16 * NT <= p.n) {         // (the wave's channels are all there) nothing to look at
         f32x4 t[NT], b[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
