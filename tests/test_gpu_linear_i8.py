@@ -118,6 +118,27 @@ def test_product(rows, k, n, x, out):
     close(got, *want(q, s, w, t, b, leaky), out)
 
 
+@pytest.mark.parametrize("rows,k,n,x,out", [(33000, 512, 256, "bf16", "bf16"), (32769, 256, 255, "bf16", "f32"), (40000, 128, 128, "bf16", "bf16"),
+                                            (32768, 300, 200, "f32", "bf16"), (50001, 100, 64, "f32", "f32"), (33001, 768, 128, "bf16", "bf16"),
+                                            (35000, 650, 77, "bf16", "f32"), (33333, 384, 128, "bf16", "bf16"), (32800, 511, 129, "f32", "f32"),
+                                            (60000, 64, 255, "bf16", "bf16"), (34000, 768, 250, "bf16", "bf16")])
+def test_product_of_very_many_rows(rows, k, n, x, out):
+    """Panels of rows under weights that stay where they are; wide rows, ragged last panels, odd channels."""
+    rng = np.random.default_rng(rows)
+    bias, leaky = n % 2 == 1, k % 3 != 0
+    lay, w, t, b = layer_of(rng, n, k, bias, leaky, out)
+    wide = torch.zeros(rows, k + 24, dtype=DT[x], device="cuda")
+    xs = torch.from_numpy(rows_of(rng, rows, k)).to(DT[x])
+    xs[5, 3] = float("nan")
+    wide[:, 16:16 + k] = xs.cuda()
+    q, s = rule(xs.float().numpy())
+    got = lay(wide[:, 16:16 + k])
+    ref, size = want(q, s, w, t, b, leaky)
+    close(got, ref, size, out)
+    assert torch.isnan(got[5]).all() and not torch.isnan(got[6:]).any()
+    assert torch.equal(lay(xs.cuda()[rows - 70:]), got[rows - 70:])
+
+
 @pytest.mark.parametrize("rows,k,n", [(4100, 640, 2100), (3000, 512, 3001), (8200, 1037, 1025), (2300, 4096, 4100)])
 @pytest.mark.parametrize("x,out", [("bf16", "bf16"), ("i8", "f32"), ("i8", "bf16"), ("f32", "f32")])
 def test_product_of_many_rows_and_channels(rows, k, n, x, out):
@@ -233,7 +254,7 @@ def test_empty_and_refusals():
         lay(buf[:128].view(4, 32), out=buf[100:132].view(4, 8))
 
 
-@pytest.mark.parametrize("rows,k,n", [(1, 4096, 512), (30, 8192, 64), (361, 1024, 512), (3000, 256, 255), (1200, 2500, 600)])
+@pytest.mark.parametrize("rows,k,n", [(1, 4096, 512), (30, 8192, 64), (361, 1024, 512), (3000, 256, 255), (1200, 2500, 600), (33000, 256, 128)])
 def test_streams_and_graph_replays(rows, k, n):
     """Two layers of one input on two streams at once, then a captured run replayed on changing inputs, eager work between."""
     rng = np.random.default_rng(rows)

@@ -244,30 +244,36 @@ template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(uns
 // Float rows -> 8-bit rows in LDS.  A wave takes 64 / LPR rows at a time, LPR lanes each, a lane's CPL chunks of eight values
 // LPR chunks apart, and NB such groups at once: all their loads are in flight together, the maxima of a group are one
 // register, and lane n of every 16 divides for group n.  Rows from nr on repeat the last one.
-template <int XT, int BM, int LPR, int CPL, int REGS>
-__device__ __forceinline__ void quantize_panel(const LinArgs &p, const char *x0, int nr, char *rows_lds, int pitch, float *row_s, int wave, int lane) {
-    constexpr int ES = XT == Y3_BF16 ? 2 : 4, N = Raw<XT>::N, RG = 64 / LPR;
-    constexpr int FIT = REGS / N / CPL < 1 ? 1 : REGS / N / CPL, EACH = (BM / RG + PN_WAVES - 1) / PN_WAVES, NB0 = FIT < EACH ? FIT : EACH;
-    constexpr int NB = NB0 < 8 ? NB0 : 8;
-    const int l = lane & (LPR - 1), in_group = LPR == 64 ? 0 : lane / LPR;
-    const bool full = p.k == LPR * CPL * 8 && nr == BM;
-    const long ld = p.x_ld * ES, lane_ld = in_group * ld;
-    const int lane_pitch = in_group * pitch + l * 8;
-    for (int b0 = 0; (wave + PN_WAVES * b0) * RG < nr; b0 += NB) {
-        unsigned v[NB][CPL][N], m[NB];
-        const auto row_of = [&](int n) { return min((wave + PN_WAVES * (b0 + n)) * RG + in_group, nr - 1); };
-        // (FULL: every lane's chunks are whole and every group has its rows: nothing to look at)
-        const auto group_of = [&](int n) { return min((wave + PN_WAVES * (b0 + n)) * RG, BM - RG); };
-        const auto load = [&](auto FULL) {
+template <int XT, int WAVES, int BM, int LPR, int CPL, int REGS>
+struct FloatRows {
+    static constexpr int ES = XT == Y3_BF16 ? 2 : 4, N = Raw<XT>::N, RG = 64 / LPR;
+    static constexpr int FIT = REGS / N / CPL < 1 ? 1 : REGS / N / CPL, EACH = (BM / RG + WAVES - 1) / WAVES, NB0 = FIT < EACH ? FIT : EACH;
+    static constexpr int NB = NB0 < 8 ? NB0 : 8, BATCH = WAVES * NB * RG;        // rows that all waves take at once
+    unsigned v[NB][CPL][N];
+
+    // every lane's chunks are whole and every group has its rows: nothing to look at
+    static __device__ __forceinline__ bool full(const LinArgs &p, int nr) { return p.k == LPR * CPL * 8 && nr == BM; }
+    static __device__ __forceinline__ int group_of(int n, int row0, int wave) { return min(row0 + (wave + WAVES * n) * RG, BM - RG); }
+    static __device__ __forceinline__ int row_of(int n, int row0, int nr, int wave, int lane) {
+        return min(row0 + (wave + WAVES * n) * RG + (LPR == 64 ? 0 : lane / LPR), nr - 1);
+    }
+
+    // rows row0 .. row0 + BATCH - 1 of the panel at x0
+    template <bool FULL> __device__ __forceinline__ void load(const LinArgs &p, const char *x0, int row0, int nr, int wave, int lane) {
+        const int l = lane & (LPR - 1);
+        const long ld = p.x_ld * ES, lane_ld = (LPR == 64 ? 0 : lane / LPR) * ld;
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const char *xr = decltype(FULL)::value ? x0 + group_of(n) * ld + lane_ld : x0 + row_of(n) * ld;
+        for (int n = 0; n < NB; ++n) {
+            const char *xr = FULL ? x0 + group_of(n, row0, wave) * ld + lane_ld : x0 + row_of(n, row0, nr, wave, lane) * ld;
 #pragma unroll
-                for (int c = 0; c < CPL; ++c) Raw<XT>::load(xr, (l + c * LPR) * 8, decltype(FULL)::value ? 8 : p.k - (l + c * LPR) * 8, v[n][c]);
-            }
-        };
-        if (full) load(std::true_type{});
-        else load(std::false_type{});
+            for (int c = 0; c < CPL; ++c) Raw<XT>::load(xr, (l + c * LPR) * 8, FULL ? 8 : p.k - (l + c * LPR) * 8, v[n][c]);
+        }
+    }
+
+    // ... to LDS, with their scales.  The division is lane n's for group n.
+    template <bool FULL> __device__ __forceinline__ void quantize(int k_bytes, int row0, int nr, char *rows_lds, int pitch, float *row_s, int wave, int lane) {
+        const int l = lane & (LPR - 1), lane_pitch = (LPR == 64 ? 0 : lane / LPR) * pitch + l * 8;
+        unsigned m[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             if constexpr (XT == Y3_BF16) {
@@ -293,31 +299,182 @@ __device__ __forceinline__ void quantize_panel(const LinArgs &p, const char *x0,
             for (int n = 0; n < NB; ++n) m[n] = lanes_max<LPR>(XT == Y3_BF16 ? m[n] << 16 : m[n], [](unsigned a, unsigned b) { return max(a, b); });
         }
         unsigned mine = m[0];
-        int row = row_of(0);
+        int row = row_of(0, row0, nr, wave, lane);
 #pragma unroll
         for (int n = 1; n < NB; ++n)
-            if ((lane & 15) == n) { mine = m[n]; row = row_of(n); }
+            if ((lane & 15) == n) { mine = m[n]; row = row_of(n, row0, nr, wave, lane); }
         const RowScale r = row_scale(mine);
         if (l < NB) row_s[row] = r.s;                            // (NB <= 8 <= LPR)
         const unsigned inv_bits = __float_as_uint(r.finite ? r.inv : 0.0f);
-        const auto write = [&](auto NN, auto FULL) {
+        const auto write = [&](auto NN) {
             constexpr int n = decltype(NN)::value;
             if constexpr (n < NB) {
                 const float inv = __uint_as_float(dpp_u<0x150 + n>(inv_bits));
-                char *to = rows_lds + (decltype(FULL)::value ? group_of(n) * pitch + lane_pitch : row_of(n) * pitch + l * 8);
+                char *to = rows_lds + (FULL ? group_of(n, row0, wave) * pitch + lane_pitch : row_of(n, row0, nr, wave, lane) * pitch + l * 8);
 #pragma unroll
                 for (int c = 0; c < CPL; ++c)
-                    if (decltype(FULL)::value || (l + c * LPR) * 8 < p.kb * 64) *(unsigned long long *)(to + c * LPR * 8) = Raw<XT>::quantize(v[n][c], inv);
+                    if (FULL || (l + c * LPR) * 8 < k_bytes) *(unsigned long long *)(to + c * LPR * 8) = Raw<XT>::quantize(v[n][c], inv);
+                __builtin_amdgcn_sched_barrier(0);               // (one group after the other: registers)
             }
         };
-        const auto write_all = [&](auto FULL) {
-            write(std::integral_constant<int, 0>{}, FULL); write(std::integral_constant<int, 1>{}, FULL);
-            write(std::integral_constant<int, 2>{}, FULL); write(std::integral_constant<int, 3>{}, FULL);
-            write(std::integral_constant<int, 4>{}, FULL); write(std::integral_constant<int, 5>{}, FULL);
-            write(std::integral_constant<int, 6>{}, FULL); write(std::integral_constant<int, 7>{}, FULL);
-        };
-        if (full) write_all(std::true_type{});
-        else write_all(std::false_type{});
+        write(std::integral_constant<int, 0>{}); write(std::integral_constant<int, 1>{}); write(std::integral_constant<int, 2>{});
+        write(std::integral_constant<int, 3>{}); write(std::integral_constant<int, 4>{}); write(std::integral_constant<int, 5>{});
+        write(std::integral_constant<int, 6>{}); write(std::integral_constant<int, 7>{});
+    }
+};
+
+template <int XT, int BM, int LPR, int CPL, int REGS>
+__device__ __forceinline__ void quantize_panel(const LinArgs &p, const char *x0, int nr, char *rows_lds, int pitch, float *row_s, int wave, int lane) {
+    typedef FloatRows<XT, PN_WAVES, BM, LPR, CPL, REGS> Rows;
+    Rows rows;
+    const bool full = Rows::full(p, nr);
+    for (int row0 = 0; row0 + wave * Rows::RG < nr; row0 += Rows::BATCH) {
+        if (full) rows.template load<true>(p, x0, row0, nr, wave, lane);
+        else rows.template load<false>(p, x0, row0, nr, wave, lane);
+        if (full) rows.template quantize<true>(p.kb * 64, row0, nr, rows_lds, pitch, row_s, wave, lane);
+        else rows.template quantize<false>(p.kb * 64, row0, nr, rows_lds, pitch, row_s, wave, lane);
+    }
+}
+
+// The wave's 16 RT x 16 NT block: scaled, activated and stored.  base: element (first row, first channel) of the block, the same
+// in all lanes; row_bytes * 64 is below 2 GB; s(r): the scale of this lane's row of 16-row block r; rows: how many rows of the
+// block there are; channels: of its channels, those that exist.
+template <int RT, int NT, bool F32, typename S>
+__device__ __forceinline__ void store_block(const LinArgs &p, char *base, int frow, int fq, const i32x4 (&acc)[RT][NT], const f32x4 (&t)[NT], const f32x4 (&b)[NT],
+                                            int rows, int channels, S s) {
+    constexpr int ES = F32 ? 4 : 2;
+    const unsigned row_bytes = (unsigned)p.out_ld * ES, lane_row = (unsigned)frow * row_bytes;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        f32x4 y[NT];
+        const float sr = s(r);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[i][j] = leaky_max(fmaf((float)acc[r][i][j] * t[i][j], sr, b[i][j]), p.slope);
+        if (r * 16 + frow >= rows) continue;                     // (lanes that trade places in a swap share their row)
+        char *o = base + (unsigned)(r * 16) * row_bytes;
+        if (channels < 16 * NT) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i * 16 + fq * 4 + j < channels) {
+                        if constexpr (F32) *(float *)(o + lane_row + (unsigned)(i * 16 + fq * 4 + j) * ES) = y[i][j];
+                        else *(unsigned short *)(o + lane_row + (unsigned)(i * 16 + fq * 4 + j) * ES) = f32_to_bf16(y[i][j]);
+                    }
+        } else if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) *(f32x4_u4 *)(o + (lane_row + fq * 16u) + i * 64) = y[i];
+        } else if constexpr (NT == 1) {
+            *(u64_u2 *)(o + lane_row + fq * 8u) = (unsigned long long)pack_bf16x2(y[0][2], y[0][3]) << 32 | pack_bf16x2(y[0][0], y[0][1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NT; i += 2) {                    // two blocks change places between quarter-waves: eight channels per lane
+                const auto s0 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(y[i][0], y[i][1]), pack_bf16x2(y[i + 1][0], y[i + 1][1]), false, false);
+                const auto s1 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(y[i][2], y[i][3]), pack_bf16x2(y[i + 1][2], y[i + 1][3]), false, false);
+                *(u32x4_u2 *)(o + (lane_row + ((fq & 1) ? 16 + (fq - 1) * 4 : fq * 4) * 2u) + i * 32) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+            }
+        }
+    }
+}
+
+// Resident kernel: few enough weights for the registers of a workgroup (k up to 64 KB, channels up to 64 NT), many rows.
+// Two workgroups of four waves per CU walk panels of 32 rows; a wave keeps the weights of its 16 NT channels for the whole
+// launch and one panel's float rows on their way: the next panel is requested as soon as this one is quantised, and arrives
+// under its products and stores.  LDS holds two panels, so that one barrier per panel is enough.  The two waves of a SIMD
+// belong to different workgroups, so that one's quantisation and stores (vector ALU) run beside the other's products; one
+// workgroup of eight waves and 64 rows, all in step, took 37 us for 92416 x 512 -> 256, the panel kernel 38 us.
+constexpr int RS_THREADS = 256, RS_ROWS = 32;
+
+// FULL: k = 8 LPR CPL and every panel has its rows (the launcher sees to that), so that no load looks at an end.
+template <int XT, int LPR, int CPL, int KB, int NT, bool FULL, bool F32>
+__global__ __launch_bounds__(RS_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void linear_i8_resident_kernel(const LinArgs p, int panels) {
+    constexpr int BM = RS_ROWS, RT = 2, PITCH = KB * 64 + 32, PANEL = BM * PITCH;
+    typedef FloatRows<XT, RS_THREADS / 64, BM, LPR, CPL, 1024> Rows;
+    static_assert(Rows::BATCH >= BM, "a panel at once");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float *row_s = (float *)(smem + 2 * PANEL), *col_t = row_s + 2 * BM, *col_b = col_t + RS_THREADS / 4 * NT;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int frow = lane & 15, fq = lane >> 4;
+    const int n0 = wave * 16 * NT, frags = (p.n + 15) >> 4;
+    const auto rows_at = [&](int panel) { return FULL ? BM : (int)min(p.rows - (long)panel * BM, (long)BM); };
+    const auto x_at = [&](int panel) { return p.x + (long)panel * BM * p.x_ld * (XT == Y3_BF16 ? 2 : 4); };
+
+    Rows rows;
+    const auto request = [&](int panel) {
+        const int nr = rows_at(panel);
+        rows.template load<FULL>(p, x_at(panel), 0, nr, wave, lane);
+    };
+    i32x4 wf[NT][KB];
+    for (int c = tid; c < RS_THREADS / 4 * NT; c += RS_THREADS) {            // (in LDS: registers are for the weights)
+        col_t[c] = p.w_scale[min(c, p.n - 1)];
+        col_b[c] = p.bias ? p.bias[min(c, p.n - 1)] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const char *w = p.w + (long)min(wave * NT + i, frags - 1) * p.kb * 1024 + lane * 16;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            wf[i][kb] = i32x4{0, 0, 0, 0};
+            if (kb < p.kb) wf[i][kb] = *(const i32x4 *)(w + kb * 1024);
+        }
+    }
+    const auto quantize = [&](int panel, int buf) {
+        const int nr = rows_at(panel);
+        rows.template quantize<FULL>(KB * 64, 0, nr, smem + buf * PANEL, PITCH, row_s + buf * BM, wave, lane);
+    };
+    const int step = (int)gridDim.x;
+    int panel = blockIdx.x;                                      // (the grid is at most `panels`)
+    request(panel);
+    __builtin_amdgcn_s_waitcnt(0x0f70);                          // vmcnt(0): nothing of this is waited for inside the loop
+    quantize(panel, 0);
+    if (panel + step < panels) request(panel + step);
+    // Products of this panel, then the next one's 8-bit rows (its float rows have arrived), the request for the one after
+    // it, and this panel's stores: the wait for float rows comes before stores that it would have to wait for as well.
+    // k-blocks past the end of k multiply zero weights, by whatever LDS holds there (of the panel's own pitch).
+    for (int buf = 0; panel < panels; buf ^= 1, panel += step) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        const int nr = rows_at(panel);
+        i32x4 acc[RT][NT] = {};
+        const char *xl = smem + buf * PANEL + frow * PITCH + fq * 16;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            if (kb % 2 == 0) __builtin_amdgcn_sched_barrier(0);  // (row fragments are read two k-blocks at a time, not all at once)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const i32x4 xf = *(const i32x4 *)(xl + r * 16 * PITCH + kb * 64);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) acc[r][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i][kb], xf, acc[r][i], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float s[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r] = row_s[buf * BM + r * 16 + frow];
+        if (panel + step < panels) {
+            quantize(panel + step, buf ^ 1);
+            if (panel + 2 * step < panels) request(panel + 2 * step);
+        }
+        const long m0 = (long)panel * BM;
+#pragma unroll
+        for (int i0 = 0; i0 < NT; i0 += 2) {                     // two blocks of channels at a time: registers
+            f32x4 t[2], b[2];
+            i32x4 part[RT][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                t[i] = *(const f32x4 *)(col_t + n0 + (i0 + i) * 16 + fq * 4);
+                b[i] = *(const f32x4 *)(col_b + n0 + (i0 + i) * 16 + fq * 4);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) part[r][i] = acc[r][i0 + i];
+            }
+            if (n0 + i0 * 16 < p.n)
+                store_block<RT, 2, F32>(p, p.out + (m0 * p.out_ld + n0 + i0 * 16) * (F32 ? 4 : 2), frow, fq, part, t, b, nr, p.n - n0 - i0 * 16, [&](int r) { return s[r]; });
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 }
 
@@ -492,37 +649,18 @@ void linear_i8_panel_kernel(const LinArgs p) {
     const auto put = [&](int r, int c, const i32x4 &v) {         // 16 x 16 block: rows r .. r + 15, channels c .. c + 15 of the workgroup's
         store4(p, m0 + r + frow, n0 + c + fq * 4, v, row_s[r + frow], *(const f32x4 *)(col_t + c + fq * 4), *(const f32x4 *)(col_b + c + fq * 4));
     };
-    if (WK == 1 && nr == BM && n0 + (wn + 1) * 16 * NT <= p.n) {         // (the wave's channels are all there) nothing to look at
+    if (WK == 1 && p.out_ld < (1 << 23)) {                       // (64 rows: below 2 GB)
+        if (n0 + wn * NT * 16 >= p.n) return;
         f32x4 t[NT], b[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             t[i] = *(const f32x4 *)(col_t + (wn * NT + i) * 16 + fq * 4);
             b[i] = *(const f32x4 *)(col_b + (wn * NT + i) * 16 + fq * 4);
         }
-        const long first = (m0 + frow) * p.out_ld + n0 + wn * NT * 16;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const float s = row_s[r * 16 + frow];
-            f32x4 y[NT];
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[i][j] = leaky_max(fmaf((float)acc[r][i][j] * t[i][j], s, b[i][j]), p.slope);
-            const long at = first + r * 16 * p.out_ld;
-            if (p.out_f32) {
-#pragma unroll
-                for (int i = 0; i < NT; ++i) *(f32x4_u4 *)((float *)p.out + at + i * 16 + fq * 4) = y[i];
-            } else if constexpr (NT == 1) {
-                *(u64_u2 *)((unsigned short *)p.out + at + fq * 4) = (unsigned long long)pack_bf16x2(y[0][2], y[0][3]) << 32 | pack_bf16x2(y[0][0], y[0][1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < NT; i += 2) {                // two blocks change places between quarter-waves: eight channels per lane
-                    const auto s0 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(y[i][0], y[i][1]), pack_bf16x2(y[i + 1][0], y[i + 1][1]), false, false);
-                    const auto s1 = __builtin_amdgcn_permlane16_swap(pack_bf16x2(y[i][2], y[i][3]), pack_bf16x2(y[i + 1][2], y[i + 1][3]), false, false);
-                    *(u32x4_u2 *)((unsigned short *)p.out + at + i * 16 + ((fq & 1) ? 16 + (fq - 1) * 4 : fq * 4)) = u32x4{s0[0], s1[0], s0[1], s1[1]};
-                }
-            }
-        }
+        const int c = n0 + wn * NT * 16;
+        char *base = p.out + (m0 * p.out_ld + c) * (p.out_f32 ? 4 : 2);
+        if (p.out_f32) store_block<RT, NT, true>(p, base, frow, fq, acc, t, b, nr, p.n - c, [&](int r) { return row_s[r * 16 + frow]; });
+        else store_block<RT, NT, false>(p, base, frow, fq, acc, t, b, nr, p.n - c, [&](int r) { return row_s[r * 16 + frow]; });
     } else if (WK == 1) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
@@ -585,6 +723,43 @@ template <int XT> int launch_panel(const LinArgs &a, const Panel &c, hipStream_t
     if (c.nt == 1) return launch_panel_as<XT, 4, 1, 1>(b, st);
     if (c.nt == 2) return launch_panel_as<XT, 4, 2, 1>(b, st);
     return launch_panel_as<XT, 4, 4, 1>(b, st);
+}
+
+template <int XT, int LPR, int CPL, int KB, int NT, bool FULL, bool F32>
+int launch_resident_as(const LinArgs &a, long cus, hipStream_t st) {
+    constexpr int lds = 2 * RS_ROWS * (KB * 64 + 32) + 2 * RS_ROWS * 4 + 2 * (RS_THREADS / 4 * NT) * 4;
+    static thread_local int attr_dev = -1;
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (attr_dev != dev) {
+        if (hipFuncSetAttribute((const void *)linear_i8_resident_kernel<XT, LPR, CPL, KB, NT, FULL, F32>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+            y3_set_error("linear_i8: cannot reserve %d bytes of LDS", lds);
+            return Y3_E_LAUNCH;
+        }
+        attr_dev = dev;
+    }
+    const long panels = (a.rows + RS_ROWS - 1) / RS_ROWS;
+    hipLaunchKernelGGL((linear_i8_resident_kernel<XT, LPR, CPL, KB, NT, FULL, F32>), dim3((unsigned)(panels < 2 * cus ? panels : 2 * cus)), dim3(RS_THREADS), lds, st, a, (int)panels);
+    return y3_check_launch("linear_i8 (resident)");
+}
+// Two panels per workgroup at least, and all channels and k in its registers.
+template <int XT> bool resident_ok(const LinArgs &a, long cus) {
+    return a.rows >= 2 * 2 * RS_ROWS * cus && a.rows <= RS_ROWS * 0x3fffffffl && a.n <= 256 && a.out_ld < (1 << 23) && a.kb <= (XT == Y3_BF16 && a.n <= 128 ? 12 : 8);
+}
+template <int XT, int NT, bool F32> int launch_resident(const LinArgs &a, long cus, hipStream_t st) {
+    const bool whole = a.rows % RS_ROWS == 0;
+    if (a.kb <= 2) return whole && a.k == 128 ? launch_resident_as<XT, 16, 1, 2, NT, true, F32>(a, cus, st) : launch_resident_as<XT, 16, 1, 2, NT, false, F32>(a, cus, st);
+    if (a.kb <= 4) return whole && a.k == 256 ? launch_resident_as<XT, 32, 1, 4, NT, true, F32>(a, cus, st) : launch_resident_as<XT, 32, 1, 4, NT, false, F32>(a, cus, st);
+    if constexpr (XT == Y3_BF16 && NT == 2)
+        if (a.kb > 8) return launch_resident_as<XT, 64, 2, 12, NT, false, F32>(a, cus, st);
+    return whole && a.k == 512 ? launch_resident_as<XT, 64, 1, 8, NT, true, F32>(a, cus, st) : launch_resident_as<XT, 64, 1, 8, NT, false, F32>(a, cus, st);
+}
+template <int XT, int NT> int launch_resident_out(const LinArgs &a, long cus, hipStream_t st) {
+    return a.out_f32 ? launch_resident<XT, NT, true>(a, cus, st) : launch_resident<XT, NT, false>(a, cus, st);
+}
+template <int XT> int launch_float(const LinArgs &a, const Panel &c, long cus, hipStream_t st) {
+    if (!resident_ok<XT>(a, cus)) return launch_panel<XT>(a, c, st);
+    return a.n <= 128 ? launch_resident_out<XT, 2>(a, cus, st) : launch_resident_out<XT, 4>(a, cus, st);
 }
 
 // The largest block of rows and channels that still gives every CU a workgroup (weights are read once per 16 RT rows,
@@ -738,7 +913,7 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     a.slope = d->flags & Y3_CONV_LEAKY ? 0.1f : 1.0f; a.out_f32 = d->out_dtype == Y3_F32;
     if (d->dtype != Y3_I8 && need == 0) {
         const Panel c = panel_of(d->rows, d->n, a.kb, false, cus);
-        return d->dtype == Y3_BF16 ? launch_panel<Y3_BF16>(a, c, st) : launch_panel<Y3_F32>(a, c, st);
+        return d->dtype == Y3_BF16 ? launch_float<Y3_BF16>(a, c, cus, st) : launch_float<Y3_F32>(a, c, cus, st);
     }
     if (y3_linear_i8_tile_ok(a, cus)) return y3_linear_i8_tile_launch(a, cus, st);
     return launch_panel<Y3_I8>(a, panel_of(d->rows, d->n, a.kb, true, cus), st);
