@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .linear_i8 import _on
+from .linear_i8 import _stream_of
 
 MAX_TOP = 32
 ClassProbs = collections.namedtuple("ClassProbs", "logp entropy top_ids top_logp")
@@ -72,19 +72,25 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
     else:
         raise ValueError("logits must be float32 or bfloat16, got %s" % logits.dtype)
     top, device = int(top), logits.device
+    if device.index != torch.cuda.current_device():             # launches go to the current device
+        with torch.cuda.device(device):
+            return log_probs(logits, ids, top=top, rows=rows, classes=classes, out=out)
     if rows is None:
         if classes is not None:
             raise ValueError("classes goes with rows")
         if logits.dim() < 1 or logits.shape[-1] < 1:
             raise ValueError("logits must be [..., C], got %r" % (tuple(logits.shape),))
         C, lead = logits.shape[-1], logits.shape[:-1]
-        strides = _two_strides(logits) if C == 1 or logits.stride(-1) == 1 else None
-        if strides is None:
-            logits = logits.contiguous()
-            strides = _two_strides(logits)
-        n, group, group_ld, row_ld = strides
-        if 0 in lead:
-            n, group = 0, 1
+        if len(lead) == 1 and (C == 1 or logits.stride(1) == 1):
+            n, group, group_ld, row_ld = lead[0], 1, logits.stride(0), 0
+        else:
+            strides = _two_strides(logits) if C == 1 or logits.stride(-1) == 1 else None
+            if strides is None:
+                logits = logits.contiguous()
+                strides = _two_strides(logits)
+            n, group, group_ld, row_ld = strides
+            if 0 in lead:
+                n, group = 0, 1
         extent, rows_ptr = 1 << 42, None
     else:
         if classes is None or int(classes) < 1:
@@ -106,10 +112,11 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
         ids_ptr, ids_64 = ids.data_ptr(), int(ids.dtype == torch.int64)
     if out is None:
         if rows is None:
-            logp = torch.empty(lead, dtype=torch.float32, device=device) if ids is not None else None
-            entropy = torch.empty(lead, dtype=torch.float32, device=device)
-            top_ids = torch.empty(lead + (top,), dtype=torch.int32, device=device) if top else None
-            top_logp = torch.empty(lead + (top,), dtype=torch.float32, device=device) if top else None
+            f32 = torch.float32
+            logp = logits.new_empty(lead, dtype=f32) if ids is not None else None
+            entropy = logits.new_empty(lead, dtype=f32)
+            top_ids = logits.new_empty(lead + (top,), dtype=torch.int32) if top else None
+            top_logp = logits.new_empty(lead + (top,), dtype=f32) if top else None
         else:
             logp = torch.zeros(lead, dtype=torch.float32, device=device) if ids is not None else None
             entropy = torch.zeros(lead, dtype=torch.float32, device=device)
@@ -125,14 +132,12 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
                 raise ValueError("out: expected contiguous %s %r on %s" % (dtype, tuple(shape), device))
     if n and (ids is not None or top or entropy is not None):
         dref, need = _descriptor((code, C, n, group, group_ld, row_ld, top, ids_64, extent))
-        with _on(device):
-            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-            rc = _lib.load().y3_log_probs(dref, logits.data_ptr(), rows_ptr, ids_ptr,
-                                          logp.data_ptr() if logp is not None else None,
-                                          entropy.data_ptr() if entropy is not None else None,
-                                          top_ids.data_ptr() if top else None, top_logp.data_ptr() if top else None,
-                                          ws.data_ptr() if need else None, need,
-                                          torch.cuda.current_stream(device).cuda_stream)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        rc = _lib.load().y3_log_probs(dref, logits.data_ptr(), rows_ptr, ids_ptr,
+                                      logp.data_ptr() if logp is not None else None,
+                                      entropy.data_ptr() if entropy is not None else None,
+                                      top_ids.data_ptr() if top else None, top_logp.data_ptr() if top else None,
+                                      ws.data_ptr() if need else None, need, _stream_of(device.index))
         if rc:
             _lib.check(rc)
     return ClassProbs(logp, entropy, top_ids, top_logp)
