@@ -314,7 +314,7 @@ int y3_linear_i8_pack(const y3_linear_i8_desc *desc, int w_dtype, const void *w,
 int y3_linear_i8_workspace_bytes(const y3_linear_i8_desc *desc, int64_t *bytes);
 /* x_scale[rows] with Y3_I8 rows, NULL otherwise.  8-bit rows start on 16 bytes (x_ld a multiple of 16) and may be read up
  * to k rounded up to 16.  bias[n] may be NULL.  workspace: 16-byte aligned, of this call alone until it has run.  x and
- * out must not overlap. */
+ * out must not overlap (two channel slices of one buffer do not). */
 int y3_linear_i8(const y3_linear_i8_desc *desc, const void *x, const float *x_scale, const void *w_packed,
                  const float *w_scale, const float *bias, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 
@@ -345,6 +345,14 @@ typedef struct y3_log_probs_desc {
 int y3_log_probs_workspace_bytes(const y3_log_probs_desc *desc, int64_t *bytes);
 int y3_log_probs(const y3_log_probs_desc *desc, const void *logits, const int64_t *row_offsets, const void *ids, float *logp,
                  float *entropy, int32_t *top_ids, float *top_logp, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Where the class logits of the boxes that NMS kept lie in the heads, in the row order of y3_pack_outputs (class-major):
+ * for row r < count of image b and the scale l that its box belongs to, row_offsets[l][b][r] = floats from the start of
+ * head l to its first class logit, -1 for the other scales and for rows >= count; row_classes[b][r] = its class (-1 behind
+ * the last row).  row_offsets: int64 [num_scales][batch][num_classes * max_boxes]; kept_idx / kept_count as y3_nms* wrote
+ * them.  y3_log_probs(head l, row_offsets[l], ids = row_classes) then gives each detection's class posterior. */
+int y3_detection_rows(const y3_decode_desc *desc, const int32_t *kept_idx, const int32_t *kept_count, int max_boxes,
+                      int64_t *row_offsets, int32_t *row_classes, void *stream);
 
 int y3_version(void);
 const char *y3_last_error(void);

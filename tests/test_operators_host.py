@@ -118,3 +118,41 @@ def test_log_probs_pointer_refusals(lib):
     assert call(P, None, P, P, P + 1, P, P) == -2
     d = probs(rows=0)
     assert call(None, None, None, None, None, None, None) == 0
+
+
+def test_linear_slices_of_one_buffer_are_not_an_overlap(lib):
+    """Rows of 5000 bf16 and of 50 fp32 in one buffer of 16 KB a row: side by side they pass (the call is then refused for
+    its workspace), four bytes into each other they do not."""
+    need = ctypes.c_int64(0)
+    d = linear(k=5000, n=50, x_ld=8192, out_ld=4096, rows=70000)          # k too long to be quantised on the way: a workspace
+    assert lib.y3_linear_i8_workspace_bytes(ctypes.byref(d), ctypes.byref(need)) == 0 and need.value > 0
+    call = lambda out: lib.y3_linear_i8(ctypes.byref(d), P, None, P, P, None, out, None, 0, None)  # noqa: E731
+    for out in (P + 10000, P + 16384 - 200, P + 3 * 16384 + 12000):
+        assert call(out) == -1 and b"workspace" in lib.y3_last_error()
+    for out in (P + 9996, P + 16384 - 196, P, P + 3 * 16384 + 100):
+        assert call(out) == -1 and b"overlap" in lib.y3_last_error()
+
+
+def test_detection_rows_refusals(lib):
+    d = _lib.DecodeDesc()
+    d.batch, d.num_scales, d.num_classes, d.num_anchors = 2, 2, 80, 3
+    for l in range(2):
+        d.grid_h[l] = d.grid_w[l] = 13
+        d.head_ld[l] = 256
+    call = lambda *a: lib.y3_detection_rows(ctypes.byref(d), *a, None)  # noqa: E731
+    assert call(None, P, 51, P, P) == -1 and call(P, None, 51, P, P) == -1 and call(P, P, 51, None, P) == -1 and call(P, P, 51, P, None) == -1
+    assert call(P, P, 0, P, P) == -1 and call(P, P, 257, P, P) == -1
+    assert call(P + 2, P, 51, P, P) == -2 and call(P, P, 51, P + 4, P) == -2
+    for field, v in (("batch", 0), ("num_scales", 4), ("num_classes", 97), ("num_anchors", 0)):
+        old = getattr(d, field)
+        setattr(d, field, v)
+        assert call(P, P, 51, P, P) == -1
+        setattr(d, field, old)
+    d.head_ld[1] = 254
+    assert call(P, P, 51, P, P) == -1
+
+
+def test_int8_network_wants_bf16():
+    from yolo_amd import build_model, config
+    with pytest.raises(ValueError, match="int8"):
+        build_model.Network(config.yolov3_tiny_cfg_path, 80, dtype="fp32", device="cuda:0", int8=True)

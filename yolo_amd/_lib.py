@@ -90,6 +90,7 @@ SIGNATURES = {
     "y3_linear_i8": (c_int, [ctypes.POINTER(LinearI8Desc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "y3_log_probs_workspace_bytes": (c_int, [ctypes.POINTER(LogProbsDesc), ctypes.POINTER(ctypes.c_int64)]),
     "y3_log_probs": (c_int, [ctypes.POINTER(LogProbsDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "y3_detection_rows": (c_int, [ctypes.POINTER(DecodeDesc), c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
     "y3_version": (c_int, []),
     "y3_last_error": (ctypes.c_char_p, []),
 }

@@ -23,6 +23,7 @@ import torch
 
 from . import _lib, config, planner
 from . import darknet_weights as dw
+from .linear_i8 import Int8Linear
 from .planner import unique_config_sections  # noqa: F401  (re-exported: reference API)
 
 _NETWORKS = weakref.WeakSet()   # what tf.global_variables() is to the reference's load_weights call: the networks that
@@ -140,6 +141,34 @@ class _CompiledPlan(object):
         _lib.check(lib.y3_conv_splitk_plan(ctypes.byref(d), ctypes.byref(splits), ctypes.byref(ws_bytes)))
         return int(ws_bytes.value) if splits.value > 1 else 0
 
+    @staticmethod
+    def _int8_op(op):
+        """A 1x1 convolution that is a plain product of pixels by channels (nothing added, pooled or upsampled)."""
+        return (op["ksize"] == 1 and op["stride"] == 1 and op["res"] is None and not op["ups"] and not op.get("pool")
+                and not op["in_f32"])
+
+    def _prepare_int8(self, net, op, x, y):
+        """y3_linear_i8 in place of the convolution: rows = pixels, quantised one by one; weights per output channel."""
+        lib = _lib.load()
+        layer = net.int8_layer(op["layer"])
+        d = _lib.LinearI8Desc()
+        d.dtype, d.out_dtype = _lib.Y3_BF16, _lib.Y3_F32 if op["out_f32"] else _lib.Y3_BF16
+        d.k, d.n, d.k_pad, d.n_pad = layer.k, layer.n, layer._k_pad, layer._n_pad
+        d.rows = self.plan.batch * op["out_hw"][0] * op["out_hw"][1]
+        d.x_ld, d.out_ld = op["x"]["ld"], op["y"]["ld"]
+        d.flags = _lib.CONV_LEAKY if op["leaky"] else 0
+        need = ctypes.c_int64(0)
+        _lib.check(lib.y3_linear_i8_workspace_bytes(ctypes.byref(d), ctypes.byref(need)))
+        nbytes, dref, fn = int(need.value), ctypes.byref(d), lib.y3_linear_i8
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=net.device) if nbytes else None
+        wsp = ws.data_ptr() if nbytes else None
+        w, scale, bias = layer._weights
+        op["kernel"], op["int8"] = "linear_i8", True
+
+        def launch(env, _keep=(d, layer, ws)):
+            return fn(dref, x(env), None, w, scale, bias, y(env), wsp, nbytes, env["stream"])
+        return launch
+
     def _ptr(self, ref, es):
         """-> (kind, base_offset_bytes)"""
         buf = ref["buf"]
@@ -196,6 +225,8 @@ class _CompiledPlan(object):
             r = resolver(op["res"]) if op["res"] is not None else (lambda env: None)
             wp, bp, zp = w.data_ptr(), bias.data_ptr(), net._zeros.data_ptr()
             fn = lib.y3_conv2d_fused
+            if net.int8 and self._int8_op(op):
+                return self._prepare_int8(net, op, x, y)
             if net.splitk:              # small-batch mode: launches with few tiles and a long k are split over k
                 splits, ws_bytes = ctypes.c_int32(1), ctypes.c_int64(0)
                 _lib.check(lib.y3_conv_splitk_plan(dref, ctypes.byref(splits), ctypes.byref(ws_bytes)))
@@ -308,7 +339,7 @@ class Network(object):
     """The compiled detector: cfg layers + packed device weights + cached launch plans."""
 
     def __init__(self, config_path, num_classes, dtype=None, device=None, fuse=True, pad_input=False, stem=True,
-                 snake=None, splitk=False, resblock=None, balanced=None):
+                 snake=None, splitk=False, resblock=None, balanced=None, int8=False):
         self.config_path = config_path
         self.num_classes = num_classes
         self.dtype = dtype or config.compute_dtype
@@ -327,6 +358,11 @@ class Network(object):
         # y3_conv2d_fused_ws for the launches that leave a partial round of 256 x 256 tiles: same bits, but measured 16 - 20 %
         # SLOWER per layer inside the network (profiles/r03l), so off unless asked for (YOLO_AMD_BALANCED=1: A/B)
         self.balanced = (os.environ.get("YOLO_AMD_BALANCED", "0") == "1") if balanced is None else bool(balanced)
+        # 8-bit products (linear_i8.py) for the 1x1 convolutions that are launches of their own, the heads included: pixels
+        # quantised one by one, weights per output channel, sums exact; everything else stays as it is
+        self.int8 = bool(int8)
+        if self.int8 and self.dtype != "bf16":
+            raise ValueError("int8 goes with dtype 'bf16' (what surrounds the 8-bit products)")
         # residual blocks (1x1 -> 3x3 -> shortcut) as one launch: None = where the planner finds it pays (bf16, large
         # launches), False = never; YOLO_AMD_RESBLOCK=0 for A/B runs.  Same bits either way.
         if resblock is None and os.environ.get("YOLO_AMD_RESBLOCK") == "0":
@@ -336,6 +372,7 @@ class Network(object):
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         self.params = None
         self._packed = None
+        self._int8_layers = {}
         self._plans = {}
         self._zeros = None
         _lib.load()                 # fail now, loudly, if the HIP library is not built
@@ -359,8 +396,19 @@ class Network(object):
                 packed[li] = pack_conv(kernel, bias, self.dtype, li == first_conv, self.device)
         self.params = params
         self._packed = packed
+        self._int8_layers = {}
         self._zeros = torch.zeros(256, dtype=torch.uint8, device=self.device)
         self._plans = {}
+
+    def int8_layer(self, li):
+        """The 8-bit form of 1x1 convolution `li` (folded weights quantised per output channel), made once."""
+        layer = self._int8_layers.get(li)
+        if layer is None:
+            kernel, bias = dw.fold_batch_norm(self.params[li])
+            layer = Int8Linear(torch.from_numpy(np.ascontiguousarray(kernel[0, 0].T, dtype=np.float32)),
+                               bias=np.asarray(bias, dtype=np.float32), device=self.device)
+            self._int8_layers[li] = layer
+        return layer
 
     def load_weights(self, weights_file):
         self.set_params(dw.read_weights(weights_file, self.layers))
@@ -479,13 +527,14 @@ class OutputNodes(list):
     __call__ = run
 
 
-def yolo(input_images, is_training, config_path, num_classes, dtype=None, device=None, splitk=False):
+def yolo(input_images, is_training, config_path, num_classes, dtype=None, device=None, splitk=False, int8=False):
     """Builds the network described by a Darknet cfg (reference build_model.py:36-270).
     input_images is accepted for signature parity and may be None (the reference passes a
-    placeholder); is_training must be False (inference path only)."""
+    placeholder); is_training must be False (inference path only).  int8: the 1x1 convolutions and the heads as 8-bit
+    products (with dtype "bf16"; see Network)."""
     if is_training:
         raise ValueError("yolo_amd implements the inference path only: is_training must be False")
-    net = Network(config_path, num_classes, dtype=dtype, device=device, splitk=splitk)
+    net = Network(config_path, num_classes, dtype=dtype, device=device, splitk=splitk, int8=int8)
     _NETWORKS.add(net)
     _ORDER[net] = next(_COUNTER)
     return OutputNodes(net)

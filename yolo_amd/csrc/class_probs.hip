@@ -603,6 +603,49 @@ template <int DT> int launch_probs(const ProbsArgs &a, hipStream_t st) {
     return y3_check_launch("log_probs");
 }
 
+// ---- kept boxes -> rows of logits: one workgroup per image ------------------------------------------------------------
+constexpr int MAX_CLASSES = 96;        // y3_decode's
+struct RowsArgs {
+    y3_decode_desc d;
+    const int32_t *kept_idx, *kept_count;
+    int64_t *row_offsets;
+    int32_t *row_classes;
+    int max_boxes;
+};
+__global__ __launch_bounds__(256) void detection_rows_kernel(const RowsArgs p) {
+    __shared__ int before[MAX_CLASSES + 1];                      // rows of the classes below
+    const int b = blockIdx.x, C = p.d.num_classes, K = p.max_boxes, cap = C * K;
+    if (threadIdx.x == 0) {
+        int n = 0;
+        for (int c = 0; c < C; ++c) {
+            before[c] = n;
+            n += min(max(p.kept_count[b * C + c], 0), K);
+        }
+        before[C] = n;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < cap; i += 256) {
+        const int c = i / K, k = i - c * K;
+        if (k < before[c + 1] - before[c]) {
+            const int r = before[c] + k, box = p.kept_idx[((long)b * C + c) * K + k];
+            int base = 0;
+            for (int l = 0; l < p.d.num_scales; ++l) {
+                const int n = p.d.grid_h[l] * p.d.grid_w[l] * p.d.num_anchors, at = box - base;
+                long off = -1;
+                if (at >= 0 && at < n)
+                    off = ((long)b * p.d.grid_h[l] * p.d.grid_w[l] + at / p.d.num_anchors) * p.d.head_ld[l] + at % p.d.num_anchors * (5 + C) + 5;
+                p.row_offsets[((long)l * p.d.batch + b) * cap + r] = off;
+                base += n;
+            }
+            p.row_classes[(long)b * cap + r] = c;
+        }
+        if (i >= before[C]) {                                    // rows behind the last
+            for (int l = 0; l < p.d.num_scales; ++l) p.row_offsets[((long)l * p.d.batch + b) * cap + i] = -1;
+            p.row_classes[(long)b * cap + i] = -1;
+        }
+    }
+}
+
 int check_desc(const y3_log_probs_desc *d) {
     Y3_REQUIRE(d, Y3_E_INVALID, "log_probs: null descriptor");
     Y3_REQUIRE(d->dtype == Y3_F32 || d->dtype == Y3_BF16, Y3_E_INVALID, "log_probs: dtype %d", d->dtype);
@@ -656,4 +699,20 @@ extern "C" int y3_log_probs(const y3_log_probs_desc *d, const void *logits, cons
     a.sums = (f32x4 *)workspace;
     a.keys = (unsigned long long *)((char *)workspace + d->rows * c.n * 16);
     return d->dtype == Y3_F32 ? launch_probs<Y3_F32>(a, (hipStream_t)stream) : launch_probs<Y3_BF16>(a, (hipStream_t)stream);
+}
+
+extern "C" int y3_detection_rows(const y3_decode_desc *d, const int32_t *kept_idx, const int32_t *kept_count, int max_boxes, int64_t *row_offsets,
+                                 int32_t *row_classes, void *stream) {
+    Y3_REQUIRE(d && kept_idx && kept_count && row_offsets && row_classes, Y3_E_INVALID, "detection_rows: null pointer");
+    Y3_REQUIRE(d->batch >= 1 && d->num_scales >= 1 && d->num_scales <= 3 && d->num_anchors >= 1, Y3_E_INVALID, "detection_rows: batch %d, %d scales, %d anchors", d->batch, d->num_scales, d->num_anchors);
+    Y3_REQUIRE(d->num_classes >= 1 && d->num_classes <= MAX_CLASSES, Y3_E_INVALID, "detection_rows: num_classes %d (at most %d)", d->num_classes, MAX_CLASSES);
+    Y3_REQUIRE(max_boxes >= 1 && max_boxes <= 256, Y3_E_INVALID, "detection_rows: max_boxes %d", max_boxes);
+    for (int l = 0; l < d->num_scales; ++l)
+        Y3_REQUIRE(d->grid_h[l] >= 1 && d->grid_w[l] >= 1 && d->head_ld[l] >= d->num_anchors * (5 + d->num_classes), Y3_E_INVALID, "detection_rows: scale %d: grid %d x %d, head_ld %d", l,
+                   d->grid_h[l], d->grid_w[l], d->head_ld[l]);
+    Y3_REQUIRE(((uintptr_t)kept_idx | (uintptr_t)kept_count | (uintptr_t)row_classes) % 4 == 0 && (uintptr_t)row_offsets % 8 == 0, Y3_E_ALIGN, "detection_rows: pointer not aligned");
+    RowsArgs a;
+    a.d = *d; a.kept_idx = kept_idx; a.kept_count = kept_count; a.row_offsets = row_offsets; a.row_classes = row_classes; a.max_boxes = max_boxes;
+    hipLaunchKernelGGL(detection_rows_kernel, dim3(d->batch), dim3(256), 0, (hipStream_t)stream, a);
+    return y3_check_launch("detection_rows");
 }

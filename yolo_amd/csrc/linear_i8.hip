@@ -822,6 +822,14 @@ void launch_quant(int dtype, const void *x, int64_t rows, int k, int64_t x_ld, v
 bool overlap(const void *a, long na, const void *b, long nb) {
     return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
+// Rows of a_row bytes against rows of b_row bytes, `rows` each: two channel slices of one buffer (the same pitch, apart
+// within it) do not overlap.
+bool rows_overlap(const void *a, long a_pitch, long a_row, const void *b, long b_pitch, long b_row, long rows) {
+    if (!overlap(a, (rows - 1) * a_pitch + a_row, b, (rows - 1) * b_pitch + b_row)) return false;
+    if (a_pitch != b_pitch) return true;
+    const long apart = ((long)((uintptr_t)b - (uintptr_t)a) % a_pitch + a_pitch) % a_pitch;
+    return apart < a_row || apart + b_row > a_pitch;
+}
 
 }  // namespace
 
@@ -890,13 +898,13 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     if (rc) return rc;
     Y3_REQUIRE(x && w && w_scale && out, Y3_E_INVALID, "linear_i8: null pointer");
     Y3_REQUIRE((d->dtype == Y3_I8) == (x_scale != nullptr), Y3_E_INVALID, "linear_i8: x_scale goes with 8-bit rows, and only with them");
-    Y3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Y3_E_INVALID, "linear_i8: workspace of %lld bytes, needs %lld", (long long)workspace_bytes, (long long)need);
     Y3_REQUIRE((uintptr_t)x % es_of(d->dtype) == 0 && aligned16(w) && (uintptr_t)out % es_of(d->out_dtype) == 0 && aligned16(workspace) &&
                (uintptr_t)x_scale % 4 == 0 && (uintptr_t)w_scale % 4 == 0 && (uintptr_t)bias % 4 == 0, Y3_E_ALIGN, "linear_i8: pointer not aligned");
     if (d->dtype == Y3_I8) Y3_REQUIRE(aligned16(x) && d->x_ld % 16 == 0 && d->x_ld >= round_up(d->k, 16), Y3_E_ALIGN, "linear_i8: 8-bit rows start on 16 bytes: x_ld %lld", (long long)d->x_ld);
-    const long x_bytes = ((d->rows - 1) * d->x_ld + (d->dtype == Y3_I8 ? round_up(d->k, 16) : d->k)) * es_of(d->dtype);
-    const long out_bytes = ((d->rows - 1) * d->out_ld + d->n) * es_of(d->out_dtype);
-    Y3_REQUIRE(!overlap(x, x_bytes, out, out_bytes), Y3_E_INVALID, "linear_i8: x and out overlap");
+    const int xs = es_of(d->dtype), os = es_of(d->out_dtype);
+    Y3_REQUIRE(!rows_overlap(x, d->x_ld * xs, (d->dtype == Y3_I8 ? round_up(d->k, 16) : d->k) * xs, out, d->out_ld * os, (long)d->n * os, d->rows),
+               Y3_E_INVALID, "linear_i8: x and out overlap");
+    Y3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Y3_E_INVALID, "linear_i8: workspace of %lld bytes, needs %lld", (long long)workspace_bytes, (long long)need);
     const hipStream_t st = (hipStream_t)stream;
     LinArgs a;
     a.x = (const char *)x; a.x_scale = x_scale; a.x_ld = d->x_ld; a.k16 = (int)round_up(d->k, 16);

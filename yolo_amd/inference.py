@@ -36,6 +36,9 @@ parser.add_argument("--dtype", default=None, choices=["bf16", "fp32"])
 parser.add_argument("--no_splitk", action="store_true", help="do not split small launches over k (bit-identical to the batched path)")
 parser.add_argument("--batch", type=int, default=1, help="images per step (default 1, the reference's mode): the directory is processed in "
                     "chunks of this many images; every image gets the result it gets alone (with --no_splitk bit for bit)")
+parser.add_argument("--int8", action="store_true", help="8-bit products for the 1x1 convolutions and the heads (with --dtype bf16)")
+parser.add_argument("--alternatives", type=int, default=0, metavar="K", help="also write OUT/alternatives/<stem>.txt: per detection the log "
+                    "probability of its class, the entropy, and the K likeliest classes with theirs")
 parser.add_argument("--graph", action="store_true", help="replay one captured HIP graph per image instead of launching every kernel from the host")
 
 
@@ -103,6 +106,21 @@ def detect_batch(output_nodes, images, anchors, num_classes, input_shape, image_
     det, heads = _postprocessor(anchors, num_classes, input_shape).detect(net, images, image_shape, chunk=chunk,
                                                                           want_heads=want_heads)
     return (det, heads) if want_heads else det
+
+
+def alternatives(heads, det, anchors, num_classes, input_shape, top=3):
+    """For each detection of `det` (predict_batch / detect_batch of these heads): log probability of its class given that
+    the box holds one object, entropy, and the `top` likeliest classes.  Returns class_probs.ClassProbs, padded like
+    Detections, on the GPU (PostProcessor.alternatives)."""
+    return _postprocessor(anchors, num_classes, input_shape).alternatives(heads, det, top=top)
+
+
+def alternative_lines(out_classes, logp, entropy, top_ids, top_logp):
+    """The alternatives/<stem>.txt lines, in the (reverse) order of label_lines:
+    `class,logp,entropy,class:logp,class:logp,...`."""
+    return ["%d,%.6f,%.6f" % (out_classes[i], logp[i], entropy[i])
+            + "".join(",%d:%.6f" % (c, v) for c, v in zip(top_ids[i], top_logp[i]))
+            for i in reversed(range(len(out_classes)))]
 
 
 def predict(output_nodes, anchors, num_classes, input_shape, image_shape):
@@ -212,7 +230,11 @@ def run_inference(img_path, output_dir, args):
 
     # one image per step: launches with few output tiles are split over k (1.6 -> ~1 ms per 608 image)
     output_nodes = yolo(input_images=None, is_training=False, config_path=cfg_path, num_classes=num_classes,
-                        dtype=getattr(args, "dtype", None), splitk=batch == 1 and not getattr(args, "no_splitk", False))
+                        dtype=getattr(args, "dtype", None), splitk=batch == 1 and not getattr(args, "no_splitk", False),
+                        int8=bool(getattr(args, "int8", False)))
+    n_alt = int(getattr(args, "alternatives", 0) or 0)
+    if n_alt:
+        os.makedirs(os.path.join(output_dir, "alternatives"), exist_ok=True)
     weights = getattr(args, "weights", None) or config.yolov3_weights_path
     if getattr(args, "darknet_model", None) is None and getattr(args, "weights", None) is None:
         raise NotImplementedError("only Darknet .weights are supported (pass --darknet_model 1); the TF-checkpoint "
@@ -249,14 +271,17 @@ def run_inference(img_path, output_dir, args):
             tick = time()
             graphed(hws + [hws[-1]] * (batch - n))
             triples = [graphed.image(j) for j in range(n)]
+            det, heads = graphed.det, graphed.heads
         else:
             tick = time()
-            det = detect_batch(output_nodes, staged[:n], anchors, num_classes, input_shape, np.asarray(hws))
+            det = detect_batch(output_nodes, staged[:n], anchors, num_classes, input_shape, np.asarray(hws), want_heads=n_alt > 0)
+            det, heads = det if n_alt else (det, None)
             counts = det.count.cpu().numpy()
             triples = [(det.boxes[j, :m].cpu().numpy(), det.scores[j, :m].cpu().numpy(), det.classes[j, :m].cpu().numpy())
                        for j, m in enumerate(counts)]
         tock = time()
         total_time_pred.append((tock - tick, n))
+        alt = [v.cpu().numpy() for v in alternatives(heads, det, anchors, num_classes, input_shape, top=n_alt)] if n_alt else None
         for j, (image, (out_boxes, out_scores, out_classes)) in enumerate(zip(chunk, triples)):
             x = first + j
             print("Found {} boxes for {} in {}sec".format(len(out_boxes), "img", (tock - tick) / n))
@@ -265,6 +290,9 @@ def run_inference(img_path, output_dir, args):
                 print("{} {:.4f}".format(class_names[c], out_scores[i]))
             with open(os.path.join(output_dir, "labels", file_names[x].split(".")[0] + ".txt"), "w") as fh:
                 fh.write("".join(l + "\n" for l in lines))
+            if n_alt:
+                with open(os.path.join(output_dir, "alternatives", file_names[x].split(".")[0] + ".txt"), "w") as fh:
+                    fh.write("".join(l + "\n" for l in alternative_lines(out_classes, *[v[j] for v in alt])))
             draw_detections(image, out_boxes, out_scores, out_classes, class_names, colors).save(
                 os.path.join(output_dir, "images", file_names[x]), compress_level=1)
             results.append((out_boxes, out_scores, out_classes))

@@ -8,6 +8,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .class_probs import ClassProbs, log_probs
 
 
 def anchor_masks(num_output_layers):
@@ -208,3 +209,36 @@ class PostProcessor(object):
         """heads: list of 2 or 3 head tensors [B,g,g,A*(5+C)] (coarse first);
         image_shapes: (h, w) for all images or a [B,2] array (inference.py:218)."""
         return self.launch(*self.prepare(heads, image_shapes))
+
+    def alternatives(self, heads, det, top=3):
+        """What else each detection could be: for every row of `det` (the Detections of these heads) the log probability of
+        its class given that the box holds one object (class_probs), the entropy of that choice, and the `top` likeliest
+        classes with their log probabilities.  heads: the head tensors `det` was made from.  Returns ClassProbs of
+        [B, cap] and [B, cap, top] tensors on the GPU; rows from count[b] on hold 0, and class -1.  No host
+        synchronisation."""
+        views = [_head_view(h) for h in heads]
+        B, device, C, K = views[0][0].shape[0], views[0][0].device, self.num_classes, self.max_boxes
+        A, cap = len(anchor_masks(len(views))[0]), C * K
+        top = int(top)
+        if not 1 <= top <= min(32, C):
+            raise ValueError("top = %d: 1 .. %d" % (top, min(32, C)))
+        if tuple(det.kept_idx.shape) != (B, C, K) or det.kept_idx.device != device:
+            raise ValueError("det holds %r kept boxes, expected %r" % (tuple(det.kept_idx.shape), (B, C, K)))
+        for l, (t, _) in enumerate(views):
+            if t.shape[0] != B or t.shape[3] != A * (5 + C):
+                raise ValueError("head %d has shape %r, expected [%d, g, g, %d]" % (l, tuple(t.shape), B, A * (5 + C)))
+        d = self.describe(B, [(t.shape[1], t.shape[2], ld) for t, ld in views])
+        if det.records.shape[1] != d.boxes_per_image:
+            raise ValueError("det pools %d boxes per image, these heads %d" % (det.records.shape[1], d.boxes_per_image))
+        offsets = torch.empty((len(views), B * cap), dtype=torch.int64, device=device)
+        classes = torch.empty(B * cap, dtype=torch.int32, device=device)
+        out = ClassProbs(torch.zeros(B * cap, device=device), torch.zeros(B * cap, device=device),
+                         torch.full((B * cap, top), -1, dtype=torch.int32, device=device), torch.zeros((B * cap, top), device=device))
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().y3_detection_rows(ctypes.byref(d), det.kept_idx.data_ptr(), det.kept_count.data_ptr(), K,
+                                                     offsets.data_ptr(), classes.data_ptr(),
+                                                     torch.cuda.current_stream(device).cuda_stream))
+            for l, (t, ld) in enumerate(views):
+                flat = t.as_strided(((t.shape[0] * t.shape[1] * t.shape[2] - 1) * ld + t.shape[3],), (1,))
+                log_probs(flat, classes, top=top, rows=offsets[l], classes=C, out=out)
+        return ClassProbs(out.logp.view(B, cap), out.entropy.view(B, cap), out.top_ids.view(B, cap, top), out.top_logp.view(B, cap, top))
