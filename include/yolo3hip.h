@@ -285,10 +285,10 @@ int y3_cast_bf16_to_f32(const void *in, float *out, int64_t n, void *stream);
 /* ---- products in 8-bit integers --------------------------------------------------------
  * y[m][n] = act(s[m] * t[n] * sum_k q[m][k] * w[n][k] + bias[n]): a 1x1 convolution (build_model.py:113-179) over
  * rows = pixels, or any linear layer over rows = tokens, with one scale per row and one per output channel.
- * A row x is held as q = round_half_even(x * (127 / a)), s = a / 127, a = max(max_k |x_k|, 127 * 2^-126); a row with a
- * NaN or an infinity gets s = NaN and q = 0, so that every product of it is NaN.  The sum is exact (32-bit integers;
- * k <= 131071), hence the result does not depend on how the work is split.  act: identity, or leaky-ReLU (alpha = 0.1)
- * with Y3_CONV_LEAKY.  No padding channel of `out` is written. */
+ * A row x is held as q = round_half_even(x * (127 * (1 / a))), s = a / 127, a = max(max_k |x_k|, 127 * 2^-126), each
+ * operation rounded to fp32; a row with a NaN or an infinity gets s = NaN, so that every product of it is NaN.  The sum is
+ * exact (32-bit integers; k <= 131071), hence the result does not depend on how the work is split.  act: identity, or
+ * leaky-ReLU (alpha = 0.1) with Y3_CONV_LEAKY.  No padding channel of `out` is written. */
 typedef struct y3_linear_i8_desc {
     int32_t dtype;        /* type of x: Y3_F32 / Y3_BF16 (rows are quantised on the way), Y3_I8 (with x_scale)      */
     int32_t out_dtype;    /* Y3_F32 or Y3_BF16                                                                     */
@@ -300,8 +300,8 @@ typedef struct y3_linear_i8_desc {
     int32_t reserved;
 } y3_linear_i8_desc;
 
-/* x [rows][x_ld] (Y3_F32, Y3_BF16) -> q: 8-bit rows q_ld bytes apart, zero filled from k to the next multiple of 16, and
- * scale[rows].  q is 16-byte aligned, q_ld a multiple of 16.  Y3_I8 copies rows to that pitch (scale may be NULL). */
+/* x [rows][x_ld] (Y3_F32, Y3_BF16) -> q: 8-bit rows q_ld bytes apart, zero filled from k to the next multiple of 16 (a row
+ * that is not finite is all zeros), and scale[rows].  q is 16-byte aligned, q_ld a multiple of 16.  Y3_I8 copies rows to that pitch (scale may be NULL). */
 int y3_quantize_rows_i8(int dtype, const void *x, int64_t rows, int k, int64_t x_ld, void *q, int64_t q_ld, float *scale,
                         void *stream);
 /* Host only: fills k_pad and n_pad from k and n.  The packed weights take k_pad * n_pad bytes. */

@@ -21,7 +21,7 @@ def rule(x):
     x = np.asarray(x, dtype=np.float32)
     a = np.maximum(np.abs(x).max(axis=1), TINY)
     with np.errstate(invalid="ignore", over="ignore"):
-        q = np.rint(x * (np.float32(127) / a)[:, None])
+        q = np.rint(x * (np.float32(127) * (np.float32(1) / a))[:, None])
     bad = ~np.isfinite(x).all(axis=1)
     q[bad] = 0
     s = a / np.float32(127)
@@ -70,7 +70,7 @@ def test_quantize_rows(dt, rows, k):
     assert q.dtype == torch.int8 and q.shape == (rows, k) and s.shape == (rows,)
     np.testing.assert_array_equal(q.cpu().numpy(), wq)
     np.testing.assert_array_equal(s.cpu().numpy(), ws)
-    # what the pair stands for is within half a step of x (127 steps, three roundings of the quotient)
+    # what the pair stands for is within half a step of x (127 steps, four roundings of the quotient)
     step = ws.astype(np.float64)[:, None]
     assert (np.abs(wq * step - x.double().numpy()) <= step * (0.5 + 127 * 4 * U)).all()
 
@@ -322,5 +322,5 @@ def test_workspace_too_small_is_refused():
     assert need.value > 0
     t = torch.zeros(16, device="cuda")
     p = t.data_ptr()
-    assert lib.y3_linear_i8(ctypes.byref(d), p, None, p, p, None, p, p, need.value - 1, None) == -1
+    assert lib.y3_linear_i8(ctypes.byref(d), p, None, p, p, None, p + (1 << 40), p, need.value - 1, None) == -1      # (never touched)
     assert b"workspace" in lib.y3_last_error()

@@ -1,7 +1,7 @@
 // Matrix product in 8-bit integers with one scale per row of the input (a pixel of a 1x1 convolution, a token) and one
 // per output channel, for gfx950 (MI355X): y3_quantize_rows_i8, y3_linear_i8_layout / _pack / _workspace_bytes, y3_linear_i8.
 //
-//   s_m = max(max_k |x_mk|, 127 * 2^-126) / 127        q_mk = round_half_even(x_mk * (127 / max_k |x_mk|))
+//   a_m = max(max_k |x_mk|, 127 * 2^-126)    s_m = a_m / 127    q_mk = round_half_even(x_mk * (127 * (1 / a_m)))
 //   y_mn = act((float(sum_k q_mk w_nk) * t_n) * s_m + b_n)
 //
 // The sum is exact: v_mfma_i32_16x16x64_i8 accumulates in 32-bit integers and 128^2 * k < 2^31 for every k accepted, so no
@@ -108,7 +108,7 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
     r.finite = amax_bits < 0x7f800000u;
     const float a = fmaxf(__uint_as_float(amax_bits), QTINY);
     r.s = r.finite ? a / 127.0f : __builtin_nanf("");       // a row with a NaN or an infinity: every product of it is NaN
-    r.inv = 127.0f / a;
+    r.inv = 127.0f * (1.0f / a);                            // (two roundings: the definition)
     return r;
 }
 

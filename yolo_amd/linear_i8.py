@@ -6,8 +6,8 @@ output channel (y3_linear_i8, include/yolo3hip.h):
     rows = quantize_rows(x)                           once, for several layers:
     y1, y2 = layer1(rows.values, scale=rows.scale), layer2(rows.values, scale=rows.scale)
 
-    y[m, n] = act(s[m] t[n] sum_k q[m, k] w[n, k] + bias[n]),   q = round_half_even(x * (127 / a)),  s = a / 127,
-    a = max(max_k |x_k|, 127 * 2^-126)
+    y[m, n] = act(s[m] t[n] sum_k q[m, k] w[n, k] + bias[n]),
+    q = round_half_even(x * (127 * (1 / a))),  s = a / 127,  a = max(max_k |x_k|, 127 * 2^-126)   (in fp32)
 
 The sum is exact, so a row's result does not depend on the rows beside it.  A row with a NaN or an infinity gives NaN.
 `Network(..., int8=True)` runs its 1x1 convolutions this way.  Calls are asynchronous on the current stream of the
