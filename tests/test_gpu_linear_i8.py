@@ -139,6 +139,25 @@ def test_product_of_very_many_rows(rows, k, n, x, out):
     assert torch.equal(lay(xs.cuda()[rows - 70:]), got[rows - 70:])
 
 
+@pytest.mark.parametrize("rows,k,n", [(10001, 200, 520), (16500, 700, 3001), (9003, 120, 1000), (5000, 130, 1500), (3700, 2300, 1040), (10100, 600, 300), (500, 500, 2000),
+                                     (130, 2600, 4000), (6000, 400, 200)])
+@pytest.mark.parametrize("x,out", [("bf16", "bf16"), ("i8", "f32"), ("f32", "f32")])
+def test_product_of_the_middle_range(rows, k, n, x, out):
+    """Blocks of 32, 48 and 64 rows by one to four blocks of channels a wave; ragged last ones."""
+    rng = np.random.default_rng(rows + n)
+    bias, leaky = rows % 2 == 1, k % 200 == 0
+    lay, w, t, b = layer_of(rng, n, k, bias, leaky, out)
+    if x == "i8":
+        q = rng.integers(-128, 128, (rows, k))
+        s = np.exp(rng.normal(size=rows)).astype(np.float32)
+        got = lay(torch.from_numpy(q.astype(np.int8)).cuda(), scale=torch.from_numpy(s).cuda())
+    else:
+        xs = torch.from_numpy(rows_of(rng, rows, k)).to(DT[x])
+        q, s = rule(xs.float().numpy())
+        got = lay(xs.cuda())
+    close(got, *want(q, s, w, t, b, leaky), out)
+
+
 @pytest.mark.parametrize("rows,k,n", [(4100, 640, 2100), (3000, 512, 3001), (8200, 1037, 1025), (2300, 4096, 4100)])
 @pytest.mark.parametrize("x,out", [("bf16", "bf16"), ("i8", "f32"), ("i8", "bf16"), ("f32", "f32")])
 def test_product_of_many_rows_and_channels(rows, k, n, x, out):

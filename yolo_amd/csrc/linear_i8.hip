@@ -129,38 +129,66 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
     return v;
 }
 
+// Maximum over the LPR lanes of a row, in all of them: DPP within 16, then the halves of 32 and 64 side by side.
+template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(unsigned v, F f) {
+    v = f(v, dpp_u<0xB1>(v));
+    v = f(v, dpp_u<0x4E>(v));
+    v = f(v, dpp_u<0x141>(v));
+    v = f(v, dpp_u<0x140>(v));
+    if constexpr (LPR >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = f(s[0], s[1]);
+    }
+    if constexpr (LPR >= 64) {
+        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = f(s[0], s[1]);
+    }
+    return v;
+}
+
 // ---- rows -> 8-bit rows + scales --------------------------------------------------------------------------------
-// One workgroup of TPR threads per row, the row read twice (the second time from cache).
-template <int DT, int TPR>
-__global__ __launch_bounds__(TPR) void quant_rows_kernel(const char *x, long x_ld, long rows, int k, char *q, long q_ld, int k_fill, float *scale) {
-    __shared__ unsigned red[TPR / 64];
-    for (long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const char *xr = x + row * x_ld * (DT == Y3_BF16 ? 2 : 4);
-    char *qr = q + row * q_ld;
-    unsigned m = 0;
-    for (int k0 = threadIdx.x * 8; k0 < k; k0 += TPR * 8) {
-        unsigned v[8];
-        Chunk<DT>::load(xr, k0, k - k0, v);
-        m = amax8(v, m);
-    }
-    m = wave_umax(m);
-    if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-        __syncthreads();
-        m = red[0];
+// TPR threads per row, 256 / TPR rows per workgroup (TPR = 64: a wave each), a thread's NI chunks kept in registers between
+// the maximum and the division; rows of more than 8 TPR NI values are read twice, the second time from cache.
+template <int DT, int TPR, int NI>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void quant_rows_kernel(const char *x, long x_ld, long rows, int k, char *q, long q_ld, int k_fill, float *scale) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1, WAVES = TPR / 64;
+    __shared__ unsigned red[RPB * WAVES];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    for (long row0 = (long)blockIdx.x * RPB; row0 < rows; row0 += (long)gridDim.x * RPB) {
+        const long row = min(row0 + sub, rows - 1);                // (a row past the end: the last one once more, the same bytes)
+        const char *xr = x + row * x_ld * (DT == Y3_BF16 ? 2 : 4);
+        char *qr = q + row * q_ld;
+        unsigned v[NI][Raw<DT>::N], m = 0;
+        const auto fetch = [&](int g) {
 #pragma unroll
-        for (int w = 1; w < TPR / 64; ++w) m = max(m, red[w]);
-    }
-    const RowScale r = row_scale(m);
-    for (int k0 = threadIdx.x * 8; k0 < k_fill; k0 += TPR * 8) {
-        unsigned v[8];
-        Chunk<DT>::load(xr, k0, k - k0, v);
-        unsigned lo = q4(v[0], v[1], v[2], v[3], r.inv), hi = q4(v[4], v[5], v[6], v[7], r.inv);
-        if (!r.finite) lo = hi = 0;
-        *(unsigned long long *)(qr + k0) = (unsigned long long)hi << 32 | lo;
-    }
-    if (threadIdx.x == 0) scale[row] = r.s;
-    __syncthreads();                                        // (red is written again)
+            for (int i = 0; i < NI; ++i) {
+                const int k0 = (g + i * TPR + t) * 8;
+                Raw<DT>::load(xr, k0, k - k0, v[i]);
+            }
+        };
+        for (int g = 0; g * 8 < k; g += NI * TPR) {
+            fetch(g);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) m = max(m, Raw<DT>::amax(v[i]));
+        }
+        m = lanes_max<64>(m, [](unsigned a, unsigned b) { return max(a, b); });
+        if constexpr (WAVES > 1) {
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) m = max(m, red[w]);
+            __syncthreads();                                        // (red is written again)
+        }
+        const RowScale r = row_scale(m);
+        for (int g = 0; g * 8 < k_fill; g += NI * TPR) {
+            if (k_fill > NI * TPR * 8) fetch(g);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int k0 = (g + i * TPR + t) * 8;
+                if (k0 < k_fill) *(unsigned long long *)(qr + k0) = r.finite ? Raw<DT>::quantize(v[i], r.inv) : 0;
+            }
+        }
+        if (t == 0) scale[row] = r.s;
     }
 }
 
@@ -223,23 +251,7 @@ __global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld,
 //   per channel its scale and bias; the area of the rows is used again for the sums of the waves along k.
 constexpr int PN_THREADS = 512, PN_WAVES = 8;
 constexpr int PN_LDS_MAX = 160 * 1024;
-
-// Maximum over the LPR lanes of a row, in all of them: DPP within 16, then the halves of 32 and 64 side by side.
-template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(unsigned v, F f) {
-    v = f(v, dpp_u<0xB1>(v));
-    v = f(v, dpp_u<0x4E>(v));
-    v = f(v, dpp_u<0x141>(v));
-    v = f(v, dpp_u<0x140>(v));
-    if constexpr (LPR >= 32) {
-        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-        v = f(s[0], s[1]);
-    }
-    if constexpr (LPR >= 64) {
-        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        v = f(s[0], s[1]);
-    }
-    return v;
-}
+constexpr int pn_slab(int nt) { return nt == 4 ? 32 * 1024 : 64 * 1024; }        // bytes of a slab of 8-bit rows: two workgroups per CU, registers
 
 // Float rows -> 8-bit rows in LDS.  A wave takes 64 / LPR rows at a time, LPR lanes each, a lane's CPL chunks of eight values
 // LPR chunks apart, and NB such groups at once: all their loads are in flight together, the maxima of a group are one
@@ -478,8 +490,9 @@ void linear_i8_resident_kernel(const LinArgs p, int panels) {
     }
 }
 
+// (registers: the widest kernels and those with fp32 rows in flight take two workgroups per CU, the others three)
 template <int XT, int RT, int NT, int WK>
-__global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(NT == 4 ? 4 : 6)))
+__global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(NT == 4 || XT == Y3_I8 || (XT == Y3_F32 && RT <= 2) ? 4 : 6)))
 void linear_i8_panel_kernel(const LinArgs p) {
     constexpr int REGS = NT == 4 ? 64 : 32;                      // of float rows on their way, per lane
     constexpr int BM = 16 * RT, wn_count = PN_WAVES / WK, cols = 16 * NT * wn_count;         // rows, channels of the workgroup
@@ -491,7 +504,8 @@ void linear_i8_panel_kernel(const LinArgs p) {
     const long m0 = (long)(blockIdx.x / p.n_groups) * BM;
     const int n0 = (int)(blockIdx.x % p.n_groups) * cols;
     const int nr = (int)(p.rows - m0 < BM ? p.rows - m0 : BM);   // rows that are there
-    const int area = max(BM * pitch, WK > 1 ? PN_WAVES * RT * NT * 1024 : 0);
+    constexpr bool DIRECT = XT == Y3_I8 && WK > 1;               // few 8-bit rows: their fragments straight from memory, no panel
+    const int area = max(DIRECT ? 0 : BM * pitch, WK > 1 ? PN_WAVES * RT * NT * 1024 : 0);
     float *row_s = (float *)(smem + area), *row_inv = row_s + BM, *col_t = row_inv + BM, *col_b = col_t + cols;
     unsigned *row_max = (unsigned *)row_inv;
 
@@ -570,17 +584,36 @@ void linear_i8_panel_kernel(const LinArgs p) {
     const auto weight = [&](int i, int kb) {
         return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_w, lane * 16, w_off[i] + (unsigned)kb * 1024u, 0));
     };
+    // 8-bit rows: a slab of k is on its way to registers while the one before it is multiplied
+    constexpr int SLAB_REGS = XT == Y3_I8 && !DIRECT ? pn_slab(NT) / PN_THREADS / 16 : 1;
+    u32x4 sv[SLAB_REGS];
+    const auto slab_chunk = [&](int j, int kbs, int &row, int &c) {         // 16 bytes c of row `row`, for this thread's j-th
+        const int i = tid + j * PN_THREADS, per_row = kbs * 4;
+        row = i / per_row;
+        c = i - row * per_row;
+        return i < nr * per_row;
+    };
+    const auto request_slab = [&](int s0) {
+        if constexpr (XT == Y3_I8 && !DIRECT) {
+            const int kbs = min(p.slab, p.kb - s0);
+#pragma unroll
+            for (int j = 0; j < SLAB_REGS; ++j) {
+                int row, c;
+                sv[j] = u32x4{0, 0, 0, 0};
+                if (slab_chunk(j, kbs, row, c) && s0 * 64 + c * 16 < p.k16) sv[j] = *(const u32x4 *)(p.x + (m0 + row) * p.x_ld + s0 * 64 + c * 16);
+            }
+        }
+    };
+    request_slab(0);
     for (int s0 = 0; s0 < p.kb; s0 += p.slab) {
         const int s_kb = min(p.slab, p.kb - s0);                 // k-blocks of this slab: an even number
         const auto slab = [&]() {
-            if constexpr (XT == Y3_I8) {
+            if constexpr (XT == Y3_I8 && !DIRECT) {
                 if (s0) __syncthreads();                         // (the previous slab has been read)
-                const int chunks = s_kb * 4;                     // 16 bytes each
-                for (int i = tid; i < nr * chunks; i += PN_THREADS) {
-                    const int row = i / chunks, c = i - row * chunks, k0 = s0 * 64 + c * 16;
-                    u32x4 v = {0, 0, 0, 0};
-                    if (k0 < p.k16) v = *(const u32x4 *)(p.x + (m0 + row) * p.x_ld + k0);
-                    *(u32x4 *)(smem + row * pitch + c * 16) = v;
+#pragma unroll
+                for (int j = 0; j < SLAB_REGS; ++j) {
+                    int row, c;
+                    if (slab_chunk(j, s_kb, row, c)) *(u32x4 *)(smem + row * pitch + c * 16) = sv[j];
                 }
             }
             __syncthreads();
@@ -593,6 +626,7 @@ void linear_i8_panel_kernel(const LinArgs p) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) wa[i] = weight(i, s0);
             slab();
+            if (s0 + p.slab < p.kb) request_slab(s0 + p.slab);
             const auto multiply = [&](const i32x4 (&f)[NT], int at) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -618,29 +652,41 @@ void linear_i8_panel_kernel(const LinArgs p) {
             static_assert(NT == 1, "waves along k have one block of channels");
             constexpr int U = 4;
             const int mine = s_kb > wk ? (s_kb - wk + WK - 1) / WK : 0;
-            i32x4 wf[2][U];
-            const auto weights = [&](int g, i32x4 (&f)[U]) {     // (past the end: any fragment, not multiplied)
+            i32x4 wf[2][U], xg[2][U][DIRECT ? RT : 1];
+            const char *xr[RT];
 #pragma unroll
-                for (int u = 0; u < U; ++u) f[u] = weight(0, min(s0 + wk + (g * U + u) * WK, p.kb - 1));
+            for (int r = 0; r < RT; ++r) xr[r] = DIRECT ? p.x + (m0 + min(r * 16 + frow, nr - 1)) * p.x_ld : nullptr;
+            const auto request = [&](int g, int buf) {           // (past the end: any fragment, not multiplied)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int kb = min(s0 + wk + (g * U + u) * WK, p.kb - 1);
+                    wf[buf][u] = weight(0, kb);
+                    if constexpr (DIRECT) {                      // (past the end of k the weights are zero: any bytes of the row)
+                        const unsigned k0 = (unsigned)min(kb * 64 + fq * 16, p.k16 - 16);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) xg[buf][u][r] = *(const i32x4 *)(xr[r] + k0);
+                    }
+                }
             };
-            weights(0, wf[0]);
-            slab();
-            const auto multiply = [&](int g, const i32x4 (&f)[U]) {
+            request(0, 0);
+            if constexpr (!DIRECT) slab();
+            const auto multiply = [&](int g, int buf) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     if (g * U + u >= mine) break;
                     const int kb = wk + (g * U + u) * WK;
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) acc[r][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[u], *(const i32x4 *)(xl[r] + kb * 64), acc[r][0], 0, 0, 0);
+                    for (int r = 0; r < RT; ++r)
+                        acc[r][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[buf][u], DIRECT ? xg[buf][u][DIRECT ? r : 0] : *(const i32x4 *)(xl[r] + kb * 64), acc[r][0], 0, 0, 0);
                 }
             };
             const int groups = (mine + U - 1) / U;
             for (int g = 0; g < groups; g += 2) {
-                if (g + 1 < groups) weights(g + 1, wf[1]);
-                multiply(g, wf[0]);
+                if (g + 1 < groups) request(g + 1, 1);
+                multiply(g, 0);
                 if (g + 1 < groups) {
-                    if (g + 2 < groups) weights(g + 2, wf[0]);
-                    multiply(g + 1, wf[1]);
+                    if (g + 2 < groups) request(g + 2, 0);
+                    multiply(g + 1, 1);
                 }
             }
         }
@@ -683,11 +729,11 @@ void linear_i8_panel_kernel(const LinArgs p) {
     }
 }
 
-int panel_area(int rt, int nt, int wk, int slab) {
-    const int rows = 16 * rt * (slab * 64 + 32), sums = wk > 1 ? PN_WAVES * rt * nt * 1024 : 0;
+int panel_area(int rt, int nt, int wk, int slab, bool direct) {
+    const int rows = direct ? 0 : 16 * rt * (slab * 64 + 32), sums = wk > 1 ? PN_WAVES * rt * nt * 1024 : 0;
     return rows > sums ? rows : sums;
 }
-int panel_lds(int rt, int nt, int wk, int slab) { return panel_area(rt, nt, wk, slab) + (2 * 16 * rt + 2 * 16 * nt * (PN_WAVES / wk)) * 4; }
+int panel_lds(int rt, int nt, int wk, int slab, bool direct) { return panel_area(rt, nt, wk, slab, direct) + (2 * 16 * rt + 2 * 16 * nt * (PN_WAVES / wk)) * 4; }
 
 template <int XT, int RT, int NT, int WK>
 int launch_panel_as(LinArgs a, hipStream_t st) {
@@ -705,7 +751,7 @@ int launch_panel_as(LinArgs a, hipStream_t st) {
     a.n_groups = (a.n + cols - 1) / cols;
     const long grid = (a.rows + 16 * RT - 1) / (16 * RT) * a.n_groups;
     Y3_REQUIRE(grid < (1 << 23), Y3_E_INVALID, "linear_i8: grid of %ld workgroups", grid);
-    hipLaunchKernelGGL((linear_i8_panel_kernel<XT, RT, NT, WK>), dim3((unsigned)grid), dim3(PN_THREADS), panel_lds(RT, NT, WK, a.slab), st, a);
+    hipLaunchKernelGGL((linear_i8_panel_kernel<XT, RT, NT, WK>), dim3((unsigned)grid), dim3(PN_THREADS), panel_lds(RT, NT, WK, a.slab, XT == Y3_I8 && WK > 1), st, a);
     return y3_check_launch("linear_i8");
 }
 
@@ -719,9 +765,10 @@ template <int XT> int launch_panel(const LinArgs &a, const Panel &c, hipStream_t
     b.slab = c.slab;
     b.fd_items = make_fastdiv(a.kb * 8);
     if (c.rt == 1) return c.wk == 2 ? launch_panel_as<XT, 1, 1, 2>(b, st) : c.wk == 4 ? launch_panel_as<XT, 1, 1, 4>(b, st) : launch_panel_as<XT, 1, 1, 8>(b, st);
-    if (c.rt == 2) return c.wk == 1 ? launch_panel_as<XT, 2, 1, 1>(b, st) : launch_panel_as<XT, 2, 1, 2>(b, st);
-    if (c.nt == 1) return launch_panel_as<XT, 4, 1, 1>(b, st);
+    if (c.rt == 2) return c.nt == 1 ? launch_panel_as<XT, 2, 1, 1>(b, st) : launch_panel_as<XT, 2, 2, 1>(b, st);
     if (c.nt == 2) return launch_panel_as<XT, 4, 2, 1>(b, st);
+    if constexpr (XT != Y3_I8)
+        if (c.rt == 3) return launch_panel_as<XT, 3, 4, 1>(b, st);
     return launch_panel_as<XT, 4, 4, 1>(b, st);
 }
 
@@ -762,10 +809,14 @@ template <int XT> int launch_float(const LinArgs &a, const Panel &c, long cus, h
     return a.n <= 128 ? launch_resident_out<XT, 2>(a, cus, st) : launch_resident_out<XT, 4>(a, cus, st);
 }
 
-// The largest block of rows and channels that still gives every CU a workgroup (weights are read once per 16 RT rows,
-// rows once per 16 NT WN channels); few rows: 16, with the waves along k.
+// The largest block of rows and channels that still gives seven CUs in ten a workgroup (weights are read once per 16 RT rows,
+// rows once per 16 NT WN channels), half of the CUs where only 16 rows with the waves along k are left. 8-bit rows, us:
+// 512 x 4096 -> 4096: RT, NT = 2, 2 (256 workgroups) 24, 4, 2 (128) 31, 4, 4 (64) 48; 2048 rows: 62, 53, 57;
+// 128 x 4096 -> 4096: 2, 1 (128) 15.7, 16 rows and two waves along k (512) 23.7; bfloat16 361 x 1024 -> 512: two waves along
+// k (184) 4.1, four (368) 4.6. 48 rows instead of 64 where the fullest CU then has fewer: 23104 x 1024 -> 512 24.3 against
+// 26.3 (96 rows, 128), 16384 rows 28.6 against 25.7 (96, 64).
 Panel panel_of(long rows, int n, int kb, bool eight_bit, long cus) {
-    static const Panel all[] = {{4, 4, 1, 0}, {4, 2, 1, 0}, {4, 1, 1, 0}, {2, 1, 1, 0}, {2, 1, 2, 0}, {1, 1, 2, 0}, {1, 1, 4, 0}, {1, 1, 8, 0}};
+    static const Panel all[] = {{4, 4, 1, 0}, {4, 2, 1, 0}, {2, 2, 1, 0}, {2, 1, 1, 0}, {1, 1, 2, 0}, {1, 1, 4, 0}, {1, 1, 8, 0}};
     Panel best = {0, 0, 0, 0};
     for (const Panel &c : all) {
         const int bm = 16 * c.rt, cols = 16 * c.nt * (PN_WAVES / c.wk);
@@ -775,11 +826,14 @@ Panel panel_of(long rows, int n, int kb, bool eight_bit, long cus) {
         Panel t = c;
         t.slab = kb;
         if (eight_bit) {
-            const int most = 64 * 1024 / bm / 64;                // (two workgroups per CU)
-            t.slab = kb < most ? kb : most;
+            const int most = pn_slab(c.nt) / bm / 64 / 2 * 2;
+            t.slab = c.wk > 1 || kb < most ? kb : most;          // (waves along k read 8-bit rows from memory)
         } else if (kb > panel_fit(bm)) continue;
         best = t;
-        if ((rows + bm - 1) / bm * ((n + cols - 1) / cols) >= cus) break;
+        const long groups = (n + cols - 1) / cols;
+        if ((rows + bm - 1) / bm * groups < (c.rt == 2 && c.nt == 1 ? cus / 2 : cus * 7 / 10)) continue;
+        if (c.nt == 4 && !eight_bit && (((rows + 47) / 48 * groups + cus - 1) / cus) * 3 < (((rows + 63) / 64 * groups + cus - 1) / cus) * 4) best.rt = 3;
+        break;
     }
     return best;
 }
@@ -790,9 +844,17 @@ int es_of(int dt) { return dt == Y3_F32 ? 4 : dt == Y3_BF16 ? 2 : 1; }
 
 // Float rows go through the panel kernel at once where its LDS holds all of k for as many rows as it takes best; otherwise
 // 8-bit rows are made in the workspace first.
+//   Up to 16 rows are quantised by every workgroup, and 64K values take one as long as a launch does (16 rows of 4096 -> 4096:
+//   7.3 us against 7.9, of 8192 -> 8192: 26 against 15.6).
+//   A tile for every CU and two million weights: a pass over the rows is little beside the product, which the tile kernel
+//   computes faster (8192 x 2048 -> 4096: 116 us against 75, 16384 x 1024 -> 2048: 62, 54; fewer weights or tiles, 32768 x
+//   1024 -> 1024: 58, 62, 65536 x 2048 -> 512: 125, 147, 4096 x 2048 -> 2048: 32, 35).
 bool fused(const y3_linear_i8_desc *d) {
     const int bm = d->rows <= 16 ? 16 : d->rows <= 32 ? 32 : 64;
-    return d->k_pad / 64 <= panel_fit(bm);
+    if (d->k_pad / 64 > panel_fit(bm)) return false;
+    if (d->rows <= 16) return d->rows * d->k_pad <= 65536;
+    const long tiles = (d->rows + 255) / 256 * ((d->n + 255) / 256);
+    return tiles < 256 || (long)d->n * d->k_pad < (1l << 21) || d->k_pad < 512;
 }
 
 int check_desc(const y3_linear_i8_desc *d) {
@@ -812,11 +874,22 @@ int check_desc(const y3_linear_i8_desc *d) {
 
 unsigned rows_grid(int64_t rows) { return (unsigned)(rows < (1 << 20) ? rows : 1 << 20); }
 
-template <int TPR>
-void launch_quant(int dtype, const void *x, int64_t rows, int k, int64_t x_ld, void *q, int64_t q_ld, int k_fill, float *scale, hipStream_t st) {
-    const unsigned grid = rows_grid(rows);
-    if (dtype == Y3_BF16) hipLaunchKernelGGL((quant_rows_kernel<Y3_BF16, TPR>), dim3(grid), dim3(TPR), 0, st, (const char *)x, (long)x_ld, (long)rows, k, (char *)q, (long)q_ld, k_fill, scale);
-    else hipLaunchKernelGGL((quant_rows_kernel<Y3_F32, TPR>), dim3(grid), dim3(TPR), 0, st, (const char *)x, (long)x_ld, (long)rows, k, (char *)q, (long)q_ld, k_fill, scale);
+template <int DT, int TPR, int NI>
+void launch_quant_as(const void *x, int64_t rows, int k, int64_t x_ld, void *q, int64_t q_ld, int k_fill, float *scale, hipStream_t st) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    hipLaunchKernelGGL((quant_rows_kernel<DT, TPR, NI>), dim3(rows_grid((rows + RPB - 1) / RPB)), dim3(TPR < 256 ? 256 : TPR), 0, st, (const char *)x, (long)x_ld, (long)rows, k,
+                       (char *)q, (long)q_ld, k_fill, scale);
+}
+// A wave per row where that fills the card; the fewer and longer the rows, the more threads each.
+template <int DT>
+void launch_quant(const void *x, int64_t rows, int k, int64_t x_ld, void *q, int64_t q_ld, int k_fill, float *scale, hipStream_t st) {
+    if (rows < 512 && k > 4096) launch_quant_as<DT, 1024, 2>(x, rows, k, x_ld, q, q_ld, k_fill, scale, st);
+    else if (k > 2048 || (rows < 2048 && k > 512)) launch_quant_as<DT, 256, 4>(x, rows, k, x_ld, q, q_ld, k_fill, scale, st);
+    else launch_quant_as<DT, 64, 4>(x, rows, k, x_ld, q, q_ld, k_fill, scale, st);
+}
+void quantize_to(int dtype, const void *x, int64_t rows, int k, int64_t x_ld, void *q, int64_t q_ld, int k_fill, float *scale, hipStream_t st) {
+    if (dtype == Y3_BF16) launch_quant<Y3_BF16>(x, rows, k, x_ld, q, q_ld, k_fill, scale, st);
+    else launch_quant<Y3_F32>(x, rows, k, x_ld, q, q_ld, k_fill, scale, st);
 }
 
 bool overlap(const void *a, long na, const void *b, long nb) {
@@ -846,7 +919,7 @@ extern "C" int y3_quantize_rows_i8(int dtype, const void *x, int64_t rows, int k
     const hipStream_t st = (hipStream_t)stream;
     const int fill = (int)round_up(k, 16);
     if (dtype == Y3_I8) hipLaunchKernelGGL(repitch_rows_kernel, dim3(rows_grid(rows)), dim3(256), 0, st, (const char *)x, (long)x_ld, (long)rows, k, (char *)q, (long)q_ld, fill);
-    else launch_quant<256>(dtype, x, rows, k, x_ld, q, q_ld, fill, scale, st);
+    else quantize_to(dtype, x, rows, k, x_ld, q, q_ld, fill, scale, st);
     return y3_check_launch("quantize_rows_i8");
 }
 
@@ -910,7 +983,7 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     a.x = (const char *)x; a.x_scale = x_scale; a.x_ld = d->x_ld; a.k16 = (int)round_up(d->k, 16);
     if (need) {
         float *s = (float *)((char *)workspace + round_up(d->rows * d->k_pad, 256));
-        launch_quant<256>(d->dtype, x, d->rows, d->k, d->x_ld, workspace, d->k_pad, d->k_pad, s, st);
+        quantize_to(d->dtype, x, d->rows, d->k, d->x_ld, workspace, d->k_pad, d->k_pad, s, st);
         rc = y3_check_launch("linear_i8 (rows)");
         if (rc) return rc;
         a.x = (const char *)workspace; a.x_scale = s; a.x_ld = d->k_pad; a.k16 = d->k_pad;
