@@ -126,6 +126,22 @@ def test_hard_rows(C, dt):
         assert ((got.top_ids[i] >= 0) & (got.top_ids[i] < C)).all() and got.top_ids[i].unique().numel() == top
 
 
+@pytest.mark.parametrize("top", [1, 2, 7])
+@pytest.mark.parametrize("C", [80, 777, 1030, 4117, 9000, 33000])
+def test_equal_largest_logits(C, top):
+    """Several classes with the row's largest logit: the first ones, whatever ran on the card before."""
+    g = torch.Generator().manual_seed(C)
+    rows = 500
+    z = torch.randn(rows, C, generator=g).to(torch.bfloat16)
+    for r in range(rows):
+        z[r, torch.randperm(C, generator=g)[: r % 12]] = 6.0
+    ids = torch.randint(0, C, (rows,), generator=g)
+    zc, ic = z.cuda(), ids.cuda()
+    for before in (100.0, -100.0):
+        log_probs(torch.full((4096, max(C, 2000)), before, device="cuda"), None, top=32)
+        check(log_probs(zc, ic, top=top), z, ids, top)
+
+
 def test_strides():
     g = torch.Generator().manual_seed(1)
     C = 80

@@ -313,7 +313,7 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
         }
         list_n = 0;
     }
-    if (top > 1) *(u32x4 *)(list + 2 * tid) = u32x4{0, 0, 0, 0};
+    if (top) *(u32x4 *)(list + 2 * tid) = u32x4{0, 0, 0, 0};
     const auto value = [&](int g, int j) {
         if constexpr (DT == Y3_F32) return __uint_as_float(raw[g][j]);
         else return __uint_as_float(j % 2 ? raw[g][j / 2] & 0xffff0000u : raw[g][j / 2] << 16);
