@@ -126,6 +126,19 @@ def test_hard_rows(C, dt):
         assert ((got.top_ids[i] >= 0) & (got.top_ids[i] < C)).all() and got.top_ids[i].unique().numel() == top
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("C", [8192, 16384, 32768, 32775, 41221, 65537])
+def test_rows_a_little_longer_than_whole_chunks(C, dt):
+    g = torch.Generator().manual_seed(C)
+    z = (3 * torch.randn(9, C + 3, generator=g)).to(DT[dt])
+    z[4, C - 20:] = 9.0
+    z[5, : C - 20] = -np.inf
+    ids = torch.randint(0, C, (9,), generator=g)
+    for top in (1, 20, 32):
+        check(log_probs(z.cuda()[:, 3:], ids.cuda(), top=top), z[:, 3:], ids, top)
+        check(log_probs(z.cuda()[:, :C], ids.cuda(), top=top), z[:, :C], ids, top)
+
+
 @pytest.mark.parametrize("top", [1, 2, 7])
 @pytest.mark.parametrize("C", [80, 777, 1030, 4117, 9000, 33000])
 def test_equal_largest_logits(C, top):

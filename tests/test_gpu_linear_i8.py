@@ -231,6 +231,21 @@ def test_product_from_one_quantisation_equals_the_product_of_rows():
         assert torch.equal(b(x), b(r.values, scale=r.scale))
 
 
+@pytest.mark.parametrize("rows,k,n", [(1, 17, 5), (2, 4141, 1048), (11, 9001, 40), (100, 5001, 64), (300, 65, 257), (7195, 1742, 178), (400, 1003, 2000),
+                                      (3000, 300, 600), (9000, 100, 300), (40, 20001, 16), (5000, 601, 2100)])
+@pytest.mark.parametrize("first,extra", [(0, 0), (1, 2), (16, 15), (5, 16)])
+def test_eight_bit_rows_anywhere(rows, k, n, first, extra):
+    """8-bit rows at odd addresses and pitches, the last one up to the end of its buffer."""
+    rng = np.random.default_rng(rows + k)
+    lay, w, t, b = layer_of(rng, n, k, True, False, "f32")
+    q = rng.integers(-128, 128, (rows, k))
+    s = np.exp(rng.normal(size=rows)).astype(np.float32)
+    flat = torch.full((first + rows * (k + extra) - extra,), 99, dtype=torch.int8, device="cuda")
+    x = flat[first:].as_strided((rows, k), (k + extra, 1))
+    x.copy_(torch.from_numpy(q.astype(np.int8)))
+    close(lay(x, scale=torch.from_numpy(s).cuda()), *want(q, s, w, t, b, False), "f32")
+
+
 def test_float_weights_are_quantised_per_channel():
     rng = np.random.default_rng(7)
     w = rows_of(rng, 40, 200)
@@ -243,6 +258,20 @@ def test_float_weights_are_quantised_per_channel():
         x = torch.from_numpy(rows_of(rng, 10, 200))
         q, s = rule(x.numpy())
         close(lay(x.cuda()), *want(q, s, wq, ws, None, False), "f32")
+
+
+def test_more_rows_than_a_grid():
+    rows, k = (1 << 27) + 77, 16
+    x = torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda")
+    for n in (1, 40):
+        if n == 40:
+            x = x[: (1 << 23) + 5]
+        w = torch.arange(n * k).view(n, k) % 7 - 3
+        lay = Int8Linear(w.to(torch.int8), scale=torch.full((n,), 2.0 ** -8), out_dtype=torch.bfloat16)
+        got = lay(x, scale=torch.ones(x.shape[0], device="cuda"))
+        for lo in range(0, x.shape[0], 1 << 24):
+            part = x[lo:lo + (1 << 24)].float() @ w.float().cuda().t() * 2.0 ** -8           # (integers below 2^24: exact)
+            assert torch.equal(got[lo:lo + (1 << 24)], part.bfloat16())
 
 
 def test_sum_at_the_ends_of_32_bits():

@@ -20,7 +20,7 @@ struct ProbsArgs {
     float *logp, *entropy, *top_logp;
     int32_t *top_ids;
     long rows, group_ld, row_ld, extent, first;
-    int classes, group, top, ids_64, fast_group, chunks, chunk_vecs;
+    int classes, group, top, ids_64, fast_group, chunks, chunk_vecs, chunk_more;
     f32x4 *sums;                       // rows of several chunks: {M, Z, S} and `top` keys per chunk
     unsigned long long *keys;
     FastDiv fd_group;                  // r / group where fast_group is set (more than one row per group, fewer than 2^31 rows)
@@ -274,8 +274,8 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     }
     const char *z = p.z + at * ES;
     const int C = p.classes, top = p.top, head = (int)((16 - ((uintptr_t)z & 15)) & 15) / ES;
-    const int whole = 1 + (C - head) / VE, v0 = chunk * p.chunk_vecs;                    // (C > 1024)
-    const int c0 = max(0, head + (v0 - 1) * VE), c1 = min(C, head + (v0 + p.chunk_vecs - 1) * VE);   // the chunk's classes
+    const int whole = 1 + (C - head) / VE, v0 = chunk * p.chunk_vecs + min(chunk, p.chunk_more), vecs = p.chunk_vecs + (chunk < p.chunk_more);   // (C > 1024)
+    const int c0 = max(0, head + (v0 - 1) * VE), c1 = min(C, head + (v0 + vecs - 1) * VE);           // the chunk's classes
     const auto first_of = [&](int g) { return head + (v0 + tid + g * STEP - 1) * VE; };
     // What a chunk does not fill holds -1e38: its exponential is 0 beside any logit above -1e37, and no NaN comes of it.
     constexpr unsigned FILL = DT == Y3_F32 ? 0xfe960000u : 0xfe96fe96u;
@@ -284,11 +284,11 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     for (int g = 0; g < NV; ++g) {
         raw[g] = u32x4{FILL, FILL, FILL, FILL};
         const int w0 = wave * 64 + g * STEP;                     // (wave-uniform: all 64 vectors are there and whole)
-        if (v0 + w0 >= 1 && w0 + 63 < p.chunk_vecs && v0 + w0 + 63 < whole) {
+        if (v0 + w0 >= 1 && w0 + 63 < vecs && v0 + w0 + 63 < whole) {
             raw[g] = *(const u32x4 *)(z + (long)(head + (v0 + w0 - 1) * VE) * ES + lane * 16);
-        } else if (w0 < p.chunk_vecs && v0 + w0 <= whole) {
+        } else if (w0 < vecs && v0 + w0 <= whole) {
             const int in = tid + g * STEP, u = v0 + in, b = first_of(g);
-            if (in < p.chunk_vecs) {
+            if (in < vecs) {
                 if (u >= 1 && u < whole) raw[g] = *(const u32x4 *)(z + (unsigned)(b * ES));
                 else if (u <= whole) {
 #pragma unroll 1
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     if (__ballot(!(fabsf(big) < 1e37f) || s.s != s.s)) {
         const auto real = [&](int g, int j) {
             const int c = first_of(g) + j;
-            return c >= c0 && c < c1 && tid + g * STEP < p.chunk_vecs ? value(g, j) : ninf;
+            return c >= c0 && c < c1 && tid + g * STEP < vecs ? value(g, j) : ninf;
         };
         unseen();
         big = ninf;
@@ -557,14 +557,16 @@ __global__ __launch_bounds__(CHUNK_THREADS) void probs_join_kernel(const ProbsAr
 }
 
 // Rows of more than 1024 classes: equal chunks of at most 32 logits per thread.
-struct Chunks { int n, vecs; };
+// Whole rounds of the threads, so that only the last chunk has any that are not filled -- unless that one would be left
+// with few: then all are equal but for one vector (29 rows of 41221, 20 alternatives, 34 vectors left: 33 us against 7).
+struct Chunks { int n, vecs, more; };
 Chunks chunks_of(const y3_log_probs_desc *d) {
-    if (d->classes <= 1024) return Chunks{0, 0};
+    if (d->classes <= 1024) return Chunks{0, 0, 0};
     const int ve = d->dtype == Y3_F32 ? 4 : 8, most = CHUNK_THREADS * 32 / ve;
     const int vecs = 1 + (d->classes + ve - 1) / ve;             // (the most an alignment makes of a row)
-    const int n = (vecs + most - 1) / most;
-    // (a multiple of the threads: all of them have the same number of vectors, but for the end of a row)
-    return Chunks{n, ((vecs + n - 1) / n + CHUNK_THREADS - 1) / CHUNK_THREADS * CHUNK_THREADS};
+    const int n = (vecs + most - 1) / most, each = (int)(((vecs + n - 1) / n + CHUNK_THREADS - 1) / CHUNK_THREADS * CHUNK_THREADS);
+    if (n == 1 || vecs - (n - 1) * each >= 2 * CHUNK_THREADS) return Chunks{n, each, 0};
+    return Chunks{n, vecs / n, vecs % n};
 }
 
 template <int DT, int L, int E> void launch_lanes(const ProbsArgs &a, hipStream_t st) {
@@ -695,7 +697,7 @@ extern "C" int y3_log_probs(const y3_log_probs_desc *d, const void *logits, cons
     if (!row_offsets && d->group > 1 && d->rows < 0x7fffffff) a.fd_group = make_fastdiv(d->group);
     a.fast_group = !row_offsets && d->group > 1 && d->rows < 0x7fffffff;
     const Chunks c = chunks_of(d);
-    a.chunks = c.n; a.chunk_vecs = c.vecs;
+    a.chunks = c.n; a.chunk_vecs = c.vecs; a.chunk_more = c.more;
     a.sums = (f32x4 *)workspace;
     a.keys = (unsigned long long *)((char *)workspace + d->rows * c.n * 16);
     return d->dtype == Y3_F32 ? launch_probs<Y3_F32>(a, (hipStream_t)stream) : launch_probs<Y3_BF16>(a, (hipStream_t)stream);

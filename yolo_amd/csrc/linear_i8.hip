@@ -192,10 +192,24 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void quant_rows_kernel(const
     }
 }
 
-// 8-bit rows of any pitch and alignment -> rows on a 16-byte pitch, zero filled
+// 8-bit rows of any pitch and alignment: 16 bytes of a row, `left` of them there
+constexpr int I8_ANY = Y3_I8 + 1;
+__device__ __forceinline__ u32x4 row16(const char *at, int left) {
+    u32x4 v = {0, 0, 0, 0};
+    if (left >= 16) __builtin_memcpy(&v, at, 16);
+    else
+#pragma unroll 1
+        for (int j = 0; j < left; ++j) {
+            const unsigned b = (unsigned)(unsigned char)at[j] << (8 * (j & 3));
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v[w] |= j >> 2 == w ? b : 0;
+        }
+    return v;
+}
+// ... -> rows on a 16-byte pitch, zero filled: a wave each
 __global__ __launch_bounds__(256) void repitch_rows_kernel(const char *x, long x_ld, long rows, int k, char *q, long q_ld, int k_fill) {
-    for (long row = blockIdx.x; row < rows; row += gridDim.x)
-        for (int k0 = threadIdx.x; k0 < k_fill; k0 += 256) q[row * q_ld + k0] = k0 < k ? x[row * x_ld + k0] : 0;
+    for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (long)gridDim.x * 4)
+        for (int k0 = (threadIdx.x & 63) * 16; k0 < k_fill; k0 += 1024) *(u32x4 *)(q + row * q_ld + k0) = row16(x + row * x_ld + k0, k - k0);
 }
 
 // rows [n][ld] of 8-bit weights -> fragments
@@ -492,7 +506,7 @@ void linear_i8_resident_kernel(const LinArgs p, int panels) {
 
 // (registers: the widest kernels and those with fp32 rows in flight take two workgroups per CU, the others three)
 template <int XT, int RT, int NT, int WK>
-__global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(NT == 4 || XT == Y3_I8 || (XT == Y3_F32 && RT <= 2) ? 4 : 6)))
+__global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(NT == 4 || XT >= Y3_I8 || (XT == Y3_F32 && RT <= 2) ? 4 : 6)))
 void linear_i8_panel_kernel(const LinArgs p) {
     constexpr int REGS = NT == 4 ? 64 : 32;                      // of float rows on their way, per lane
     constexpr int BM = 16 * RT, wn_count = PN_WAVES / WK, cols = 16 * NT * wn_count;         // rows, channels of the workgroup
@@ -521,7 +535,7 @@ void linear_i8_panel_kernel(const LinArgs p) {
         col_t[c] = p.w_scale[ch];
         col_b[c] = p.bias ? p.bias[ch] : 0.0f;
     }
-    if constexpr (XT == Y3_I8) {
+    if constexpr (XT >= Y3_I8) {
         if (tid < BM) row_s[tid] = p.x_scale[min(m0 + tid, p.rows - 1)];
     } else {
         const char *x0 = p.x + m0 * p.x_ld * (XT == Y3_BF16 ? 2 : 4);
@@ -585,7 +599,7 @@ void linear_i8_panel_kernel(const LinArgs p) {
         return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs_w, lane * 16, w_off[i] + (unsigned)kb * 1024u, 0));
     };
     // 8-bit rows: a slab of k is on its way to registers while the one before it is multiplied
-    constexpr int SLAB_REGS = XT == Y3_I8 && !DIRECT ? pn_slab(NT) / PN_THREADS / 16 : 1;
+    constexpr int SLAB_REGS = XT >= Y3_I8 && !DIRECT ? pn_slab(NT) / PN_THREADS / 16 : 1;
     u32x4 sv[SLAB_REGS];
     const auto slab_chunk = [&](int j, int kbs, int &row, int &c) {         // 16 bytes c of row `row`, for this thread's j-th
         const int i = tid + j * PN_THREADS, per_row = kbs * 4;
@@ -594,13 +608,15 @@ void linear_i8_panel_kernel(const LinArgs p) {
         return i < nr * per_row;
     };
     const auto request_slab = [&](int s0) {
-        if constexpr (XT == Y3_I8 && !DIRECT) {
+        if constexpr (XT >= Y3_I8 && !DIRECT) {
             const int kbs = min(p.slab, p.kb - s0);
 #pragma unroll
             for (int j = 0; j < SLAB_REGS; ++j) {
                 int row, c;
                 sv[j] = u32x4{0, 0, 0, 0};
-                if (slab_chunk(j, kbs, row, c) && s0 * 64 + c * 16 < p.k16) sv[j] = *(const u32x4 *)(p.x + (m0 + row) * p.x_ld + s0 * 64 + c * 16);
+                if (!slab_chunk(j, kbs, row, c) || s0 * 64 + c * 16 >= p.k) continue;
+                const char *at = p.x + (m0 + row) * p.x_ld + s0 * 64 + c * 16;
+                sv[j] = XT == I8_ANY ? row16(at, p.k - s0 * 64 - c * 16) : *(const u32x4 *)at;
             }
         }
     };
@@ -608,7 +624,7 @@ void linear_i8_panel_kernel(const LinArgs p) {
     for (int s0 = 0; s0 < p.kb; s0 += p.slab) {
         const int s_kb = min(p.slab, p.kb - s0);                 // k-blocks of this slab: an even number
         const auto slab = [&]() {
-            if constexpr (XT == Y3_I8 && !DIRECT) {
+            if constexpr (XT >= Y3_I8 && !DIRECT) {
                 if (s0) __syncthreads();                         // (the previous slab has been read)
 #pragma unroll
                 for (int j = 0; j < SLAB_REGS; ++j) {
@@ -669,7 +685,10 @@ void linear_i8_panel_kernel(const LinArgs p) {
                 }
             };
             request(0, 0);
-            if constexpr (!DIRECT) slab();
+            if constexpr (!DIRECT) {
+                slab();
+                if (s0 + p.slab < p.kb) request_slab(s0 + p.slab);
+            }
             const auto multiply = [&](int g, int buf) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
@@ -749,9 +768,17 @@ int launch_panel_as(LinArgs a, hipStream_t st) {
     }
     constexpr int cols = 16 * NT * (PN_WAVES / WK);
     a.n_groups = (a.n + cols - 1) / cols;
-    const long grid = (a.rows + 16 * RT - 1) / (16 * RT) * a.n_groups;
-    Y3_REQUIRE(grid < (1 << 23), Y3_E_INVALID, "linear_i8: grid of %ld workgroups", grid);
-    hipLaunchKernelGGL((linear_i8_panel_kernel<XT, RT, NT, WK>), dim3((unsigned)grid), dim3(PN_THREADS), panel_lds(RT, NT, WK, a.slab, XT == Y3_I8 && WK > 1), st, a);
+    constexpr bool lds_direct = XT == Y3_I8 && WK > 1;
+    const long most = ((1 << 23) - 1) / a.n_groups * 16 * RT;    // rows of a grid (fewer than 2^32 threads)
+    for (long m = 0; m < a.rows; m += most) {
+        LinArgs s = a;
+        s.rows = a.rows - m < most ? a.rows - m : most;
+        s.x += m * a.x_ld * (XT == Y3_F32 ? 4 : XT == Y3_BF16 ? 2 : 1);
+        if (XT >= Y3_I8) s.x_scale += m;
+        s.out += m * a.out_ld * (a.out_f32 ? 4 : 2);
+        hipLaunchKernelGGL((linear_i8_panel_kernel<XT, RT, NT, WK>), dim3((unsigned)((s.rows + 16 * RT - 1) / (16 * RT) * a.n_groups)), dim3(PN_THREADS),
+                           panel_lds(RT, NT, WK, a.slab, lds_direct), st, s);
+    }
     return y3_check_launch("linear_i8");
 }
 
@@ -767,7 +794,7 @@ template <int XT> int launch_panel(const LinArgs &a, const Panel &c, hipStream_t
     if (c.rt == 1) return c.wk == 2 ? launch_panel_as<XT, 1, 1, 2>(b, st) : c.wk == 4 ? launch_panel_as<XT, 1, 1, 4>(b, st) : launch_panel_as<XT, 1, 1, 8>(b, st);
     if (c.rt == 2) return c.nt == 1 ? launch_panel_as<XT, 2, 1, 1>(b, st) : launch_panel_as<XT, 2, 2, 1>(b, st);
     if (c.nt == 2) return launch_panel_as<XT, 4, 2, 1>(b, st);
-    if constexpr (XT != Y3_I8)
+    if constexpr (XT < Y3_I8)
         if (c.rt == 3) return launch_panel_as<XT, 3, 4, 1>(b, st);
     return launch_panel_as<XT, 4, 4, 1>(b, st);
 }
@@ -809,30 +836,35 @@ template <int XT> int launch_float(const LinArgs &a, const Panel &c, long cus, h
     return a.n <= 128 ? launch_resident_out<XT, 2>(a, cus, st) : launch_resident_out<XT, 4>(a, cus, st);
 }
 
-// The largest block of rows and channels that still gives seven CUs in ten a workgroup (weights are read once per 16 RT rows,
-// rows once per 16 NT WN channels), half of the CUs where only 16 rows with the waves along k are left. 8-bit rows, us:
-// 512 x 4096 -> 4096: RT, NT = 2, 2 (256 workgroups) 24, 4, 2 (128) 31, 4, 4 (64) 48; 2048 rows: 62, 53, 57;
-// 128 x 4096 -> 4096: 2, 1 (128) 15.7, 16 rows and two waves along k (512) 23.7; bfloat16 361 x 1024 -> 512: two waves along
-// k (184) 4.1, four (368) 4.6. 48 rows instead of 64 where the fullest CU then has fewer: 23104 x 1024 -> 512 24.3 against
-// 26.3 (96 rows, 128), 16384 rows 28.6 against 25.7 (96, 64).
-Panel panel_of(long rows, int n, int kb, bool eight_bit, long cus) {
+// The largest block of rows and channels (weights are read once per 16 RT rows, rows once per 16 NT WN channels) that does not
+// leave half of the waves without channels and still gives seven CUs in ten a workgroup.  RT, NT (WK), 8-bit rows, us: 512 x
+// 4096 -> 4096: 2, 2 (256 workgroups) 24, 4, 2 (128) 31, 4, 4 (64) 48; 2048 rows: 62, 53, 57.  bfloat16 rows: 361 x 1024 ->
+// 512: 1, 1, 2 (184) 4.1, 1, 1, 4 (368) 4.6; 8266 x 1717 -> 60: 1, 1, 2 11.5, 2, 1 14.7.  But
+//   4, 2 from two workgroups per CU on, where two fit the LDS: 23104 x 512 -> 255 (361) 15.6, 2, 2 13.6; 46208 x 1024 -> 256
+//   29.6, 31.9; 60000 x 1280 -> 256 (its rows fill half of the LDS) 67, 51;
+//   2, 1 from half of the CUs on, as 16 rows are all that is left: 128 x 4096 -> 4096 (128) 15.7, 1, 1, 2 (512) 23.7;
+//   3, 4 instead of 4, 4 where the fullest CU then has fewer rows (23104 x 1024 -> 512: 96 rows, 24.3, 128, 26.3; 16384: 96,
+//   28.6, 64, 25.7), or where it fits the LDS twice (60000 x 1280 -> 512: 75, 88).
+Panel panel_of(long rows, int n, int kb, int xt, long cus) {
     static const Panel all[] = {{4, 4, 1, 0}, {4, 2, 1, 0}, {2, 2, 1, 0}, {2, 1, 1, 0}, {1, 1, 2, 0}, {1, 1, 4, 0}, {1, 1, 8, 0}};
+    const auto twice = [&](int rt) { return xt >= Y3_I8 || kb <= panel_fit(16 * rt) / 2; };
+    const auto fullest = [&](int bm, long groups) { return ((rows + bm - 1) / bm * groups + cus - 1) / cus * bm; };
     Panel best = {0, 0, 0, 0};
     for (const Panel &c : all) {
         const int bm = 16 * c.rt, cols = 16 * c.nt * (PN_WAVES / c.wk);
-        if (c.nt > 1 && n <= cols / 2) continue;                 // half of the waves would have nothing
+        if (n <= cols / 2 && (c.nt > 1 || (c.wk < 8 && 2 * c.wk <= kb))) continue;
         if (c.rt > 1 && rows <= bm / 2) continue;
         if (c.wk > kb) continue;
         Panel t = c;
         t.slab = kb;
-        if (eight_bit) {
+        if (xt >= Y3_I8) {
             const int most = pn_slab(c.nt) / bm / 64 / 2 * 2;
-            t.slab = c.wk > 1 || kb < most ? kb : most;          // (waves along k read 8-bit rows from memory)
+            t.slab = (c.wk > 1 && xt == Y3_I8) || kb < most ? kb : most;     // (waves along k read aligned 8-bit rows from memory)
         } else if (kb > panel_fit(bm)) continue;
         best = t;
-        const long groups = (n + cols - 1) / cols;
-        if ((rows + bm - 1) / bm * groups < (c.rt == 2 && c.nt == 1 ? cus / 2 : cus * 7 / 10)) continue;
-        if (c.nt == 4 && !eight_bit && (((rows + 47) / 48 * groups + cus - 1) / cus) * 3 < (((rows + 63) / 64 * groups + cus - 1) / cus) * 4) best.rt = 3;
+        const long groups = (n + cols - 1) / cols, all_of = (rows + bm - 1) / bm * groups;
+        if (c.rt == 4 && c.nt == 2 ? all_of < 2 * cus || !twice(4) : all_of < (c.rt == 2 && c.nt == 1 ? cus / 2 : cus * 7 / 10)) continue;
+        if (c.nt == 4 && xt < Y3_I8 && (fullest(48, groups) < fullest(64, groups) || (!twice(4) && twice(3) && all_of >= 2 * cus))) best.rt = 3;
         break;
     }
     return best;
@@ -856,6 +888,9 @@ bool fused(const y3_linear_i8_desc *d) {
     const long tiles = (d->rows + 255) / 256 * ((d->n + 255) / 256);
     return tiles < 256 || (long)d->n * d->k_pad < (1l << 21) || d->k_pad < 512;
 }
+
+// 8-bit rows that are read 16 aligned bytes at a time, up to k16
+bool rows_aligned(const LinArgs &a) { return aligned16(a.x) && a.x_ld % 16 == 0 && a.x_ld >= a.k16; }
 
 int check_desc(const y3_linear_i8_desc *d) {
     Y3_REQUIRE(d, Y3_E_INVALID, "linear_i8: null descriptor");
@@ -918,7 +953,7 @@ extern "C" int y3_quantize_rows_i8(int dtype, const void *x, int64_t rows, int k
     Y3_REQUIRE(!overlap(x, ((rows - 1) * x_ld + k) * es_of(dtype), q, rows * q_ld), Y3_E_INVALID, "quantize_rows_i8: x and q overlap");
     const hipStream_t st = (hipStream_t)stream;
     const int fill = (int)round_up(k, 16);
-    if (dtype == Y3_I8) hipLaunchKernelGGL(repitch_rows_kernel, dim3(rows_grid(rows)), dim3(256), 0, st, (const char *)x, (long)x_ld, (long)rows, k, (char *)q, (long)q_ld, fill);
+    if (dtype == Y3_I8) hipLaunchKernelGGL(repitch_rows_kernel, dim3(rows_grid((rows + 3) / 4)), dim3(256), 0, st, (const char *)x, (long)x_ld, (long)rows, k, (char *)q, (long)q_ld, fill);
     else quantize_to(dtype, x, rows, k, x_ld, q, q_ld, fill, scale, st);
     return y3_check_launch("quantize_rows_i8");
 }
@@ -973,9 +1008,8 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     Y3_REQUIRE((d->dtype == Y3_I8) == (x_scale != nullptr), Y3_E_INVALID, "linear_i8: x_scale goes with 8-bit rows, and only with them");
     Y3_REQUIRE((uintptr_t)x % es_of(d->dtype) == 0 && aligned16(w) && (uintptr_t)out % es_of(d->out_dtype) == 0 && aligned16(workspace) &&
                (uintptr_t)x_scale % 4 == 0 && (uintptr_t)w_scale % 4 == 0 && (uintptr_t)bias % 4 == 0, Y3_E_ALIGN, "linear_i8: pointer not aligned");
-    if (d->dtype == Y3_I8) Y3_REQUIRE(aligned16(x) && d->x_ld % 16 == 0 && d->x_ld >= round_up(d->k, 16), Y3_E_ALIGN, "linear_i8: 8-bit rows start on 16 bytes: x_ld %lld", (long long)d->x_ld);
     const int xs = es_of(d->dtype), os = es_of(d->out_dtype);
-    Y3_REQUIRE(!rows_overlap(x, d->x_ld * xs, (d->dtype == Y3_I8 ? round_up(d->k, 16) : d->k) * xs, out, d->out_ld * os, (long)d->n * os, d->rows),
+    Y3_REQUIRE(!rows_overlap(x, d->x_ld * xs, (long)d->k * xs, out, d->out_ld * os, (long)d->n * os, d->rows),
                Y3_E_INVALID, "linear_i8: x and out overlap");
     Y3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Y3_E_INVALID, "linear_i8: workspace of %lld bytes, needs %lld", (long long)workspace_bytes, (long long)need);
     const hipStream_t st = (hipStream_t)stream;
@@ -993,9 +1027,10 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     a.rows = d->rows; a.out_ld = d->out_ld; a.n = d->n; a.k = d->k; a.kb = d->k_pad / 64;
     a.slope = d->flags & Y3_CONV_LEAKY ? 0.1f : 1.0f; a.out_f32 = d->out_dtype == Y3_F32;
     if (d->dtype != Y3_I8 && need == 0) {
-        const Panel c = panel_of(d->rows, d->n, a.kb, false, cus);
+        const Panel c = panel_of(d->rows, d->n, a.kb, d->dtype, cus);
         return d->dtype == Y3_BF16 ? launch_float<Y3_BF16>(a, c, cus, st) : launch_float<Y3_F32>(a, c, cus, st);
     }
+    if (!rows_aligned(a)) return launch_panel<I8_ANY>(a, panel_of(d->rows, d->n, a.kb, I8_ANY, cus), st);
     if (y3_linear_i8_tile_ok(a, cus)) return y3_linear_i8_tile_launch(a, cus, st);
-    return launch_panel<Y3_I8>(a, panel_of(d->rows, d->n, a.kb, true, cus), st);
+    return launch_panel<Y3_I8>(a, panel_of(d->rows, d->n, a.kb, Y3_I8, cus), st);
 }

@@ -46,15 +46,19 @@ def _check_input(x, name):
         raise ValueError("%s requires a gradient: the 8-bit product has none (use torch.no_grad())" % name)
 
 
-def _repitch(x):
-    """8-bit rows as the kernels read them: on 16 bytes, readable up to a multiple of 16."""
+def _eight_bit_rows(x, n):
+    """8-bit rows and their pitch as y3_linear_i8 takes them.  Rows on 16 bytes are read up to a multiple of 16, which has to
+    be there; others are read as they are, or copied where the product takes far longer than a copy (the kernel for many
+    rows and channels needs them on 16 bytes: 8192 x 8192 -> 8192 in half the time)."""
     rows, k = x.shape
     pitch = (k + 15) // 16 * 16
     ld = x.stride(0) if rows > 1 else pitch
-    if x.data_ptr() % 16 == 0 and ld % 16 == 0 and (
-            k == pitch or x.storage_offset() + (rows - 1) * ld + pitch <= x.untyped_storage().nbytes()):
+    aligned = x.data_ptr() % 16 == 0 and ld % 16 == 0 and ld >= pitch
+    if aligned and (k == pitch or x.storage_offset() + (rows - 1) * ld + pitch <= x.untyped_storage().nbytes()):
         return x, ld
     ld = x.stride(0) if rows > 1 else k
+    if not (rows > 1 and aligned) and (k < 512 or rows * n < 1 << 23):
+        return x, ld
     q = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
     _lib.check(_lib.load().y3_quantize_rows_i8(_lib.Y3_I8, x.data_ptr(), rows, k, ld, q.data_ptr(), pitch, None,
                                                _stream_of(x.device.index)))
@@ -170,7 +174,7 @@ class Int8Linear(object):
                 raise ValueError("scale must be float32 with one value per row on %s" % device)
             scale = scale.contiguous()
             scale_ptr = scale.data_ptr()
-            m, x_ld = _repitch(m)
+            m, x_ld = _eight_bit_rows(m, self.n)
         else:
             x_ld = m.stride(0) if rows > 1 else self.k
         key = (code, rows, x_ld, out_ld)
