@@ -112,11 +112,10 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
         ids_ptr, ids_64 = ids.data_ptr(), int(ids.dtype == torch.int64)
     if out is None:
         if rows is None:
-            f32 = torch.float32
-            logp = logits.new_empty(lead, dtype=f32) if ids is not None else None
-            entropy = logits.new_empty(lead, dtype=f32)
-            top_ids = logits.new_empty(lead + (top,), dtype=torch.int32) if top else None
-            top_logp = logits.new_empty(lead + (top,), dtype=f32) if top else None
+            entropy = logits.new_empty(lead, dtype=torch.float32)
+            logp = torch.empty_like(entropy) if ids is not None else None
+            top_logp = logits.new_empty(lead + (top,), dtype=torch.float32) if top else None
+            top_ids = torch.empty_like(top_logp, dtype=torch.int32) if top else None
         else:
             logp = torch.zeros(lead, dtype=torch.float32, device=device) if ids is not None else None
             entropy = torch.zeros(lead, dtype=torch.float32, device=device)
@@ -132,7 +131,7 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
                 raise ValueError("out: expected contiguous %s %r on %s" % (dtype, tuple(shape), device))
     if n and (ids is not None or top or entropy is not None):
         dref, need = _descriptor((code, C, n, group, group_ld, row_ld, top, ids_64, extent))
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        ws = logits.new_empty(need, dtype=torch.uint8) if need else None
         rc = _lib.load().y3_log_probs(dref, logits.data_ptr(), rows_ptr, ids_ptr,
                                       logp.data_ptr() if logp is not None else None,
                                       entropy.data_ptr() if entropy is not None else None,

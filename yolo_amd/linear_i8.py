@@ -157,7 +157,7 @@ class Int8Linear(object):
         rows = m.shape[0]
         shape = (rows, self.n) if m is x else x.shape[:-1] + (self.n,)
         if out is None:
-            out = torch.empty(shape, dtype=self.out_dtype, device=device)
+            out = x.new_empty(shape, dtype=self.out_dtype)
             out_ld = self.n
         else:
             if out.dtype != self.out_dtype or out.shape != shape or out.device != device:
@@ -179,7 +179,7 @@ class Int8Linear(object):
             x_ld = m.stride(0) if rows > 1 else self.k
         key = (code, rows, x_ld, out_ld)
         dref, need = self._descs.get(key) or self._desc(key)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
         w, ws_scale, b = self._weights
         rc = _lib.load().y3_linear_i8(dref, m.data_ptr(), scale_ptr, w, ws_scale, b, out.data_ptr(),
                                       ws.data_ptr() if need else None, need, _stream_of(device.index))
