@@ -274,6 +274,25 @@ def test_more_rows_than_a_grid():
             assert torch.equal(got[lo:lo + (1 << 24)], part.bfloat16())
 
 
+@pytest.mark.parametrize("k", [130, 20])
+def test_very_many_channels(k):
+    """2^24 channels: weights and outputs past 32-bit offsets."""
+    n, rows = 1 << 24, 65
+    if k == 130:                                             # 8-bit weights
+        w = torch.randint(-128, 128, (n, k), dtype=torch.int8, device="cuda")
+        lay = Int8Linear(w, scale=torch.full((n,), 2.0 ** -6, device="cuda"))
+    else:                                                    # float weights that are their own 8-bit values
+        w = torch.randint(-126, 127, (n, k), dtype=torch.int8, device="cuda")
+        w[:, 3] = 127
+        lay = Int8Linear(w.float() * 2.0 ** -6, out_dtype=torch.bfloat16)
+        assert torch.equal(lay.scale, torch.full((n,), 2.0 ** -6, device="cuda"))
+    x = torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda")
+    got = lay(x, scale=torch.ones(rows, device="cuda"))
+    for lo in range(0, n, 1 << 22):
+        part = x.float() @ w[lo:lo + (1 << 22)].float().t() * 2.0 ** -6                      # (integers below 2^24: exact)
+        assert torch.equal(got[:, lo:lo + (1 << 22)], part.bfloat16())
+
+
 def test_sum_at_the_ends_of_32_bits():
     k = 131071
     for xv, wv in ((-128, -128), (127, -128), (-128, 127)):
@@ -288,7 +307,7 @@ def test_empty_and_refusals():
     x = torch.ones(4, 32, device="cuda")
     s = torch.ones(4, device="cuda")
     for bad in (lambda: lay(x[:, :31]), lambda: lay(x.half()), lambda: lay(x.cpu()), lambda: lay(x, scale=s),
-                lambda: lay(x.to(torch.int8)), lambda: lay(x.to(torch.int8), scale=s[:3]),
+                lambda: lay(x.to(torch.int8)), lambda: lay(x.to(torch.int8), scale=s[:3]), lambda: lay(x.to(torch.int8).view(2, 2, 32), scale=s.view(1, 4)),
                 lambda: lay(x, out=torch.empty(4, 8, dtype=torch.bfloat16, device="cuda")),
                 lambda: lay(x, out=torch.empty(4, 9, device="cuda")), lambda: lay(x, out=torch.empty(8, 4, device="cuda").t()),
                 lambda: lay(x.clone().requires_grad_()), lambda: Int8Linear(torch.ones(8, 32), scale=torch.ones(8)),

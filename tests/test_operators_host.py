@@ -153,3 +153,12 @@ def test_int8_network_wants_bf16():
     from yolo_amd import build_model, config
     with pytest.raises(ValueError, match="int8"):
         build_model.Network(config.yolov3_tiny_cfg_path, 80, dtype="fp32", device="cuda:0", int8=True)
+
+
+@pytest.mark.parametrize("k", [-1, 33])
+def test_alternatives_option_range(tmp_path, k):
+    import argparse
+    from yolo_amd import inference
+    with pytest.raises(ValueError, match="alternatives"):
+        inference.run_inference(str(tmp_path), str(tmp_path / "out"), argparse.Namespace(alternatives=k))
+    assert not (tmp_path / "out").exists()

@@ -123,12 +123,6 @@ __device__ __forceinline__ unsigned q4(unsigned a, unsigned b, unsigned c, unsig
     return lo | hi;
 }
 
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
-    return v;
-}
-
 // Maximum over the LPR lanes of a row, in all of them: DPP within 16, then the halves of 32 and 64 side by side.
 template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(unsigned v, F f) {
     v = f(v, dpp_u<0xB1>(v));
@@ -214,46 +208,48 @@ __global__ __launch_bounds__(256) void repitch_rows_kernel(const char *x, long x
 
 // rows [n][ld] of 8-bit weights -> fragments
 __global__ __launch_bounds__(256) void pack_i8_kernel(const char *w, long ld, int n, int k, int kb_total, long chunks, char *packed) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;               // one 16-byte lane of a fragment
-    if (i >= chunks) return;
-    const long frag = i >> 6;
-    const int lane = (int)(i & 63), ch = (int)(frag / kb_total) * 16 + (lane & 15);
-    const int k0 = (int)(frag % kb_total) * 64 + (lane >> 4) * 16;
-    unsigned r[4] = {0, 0, 0, 0};
-    if (ch < n)
-        for (int j = 0; j < 16; ++j)
-            if (k0 + j < k) r[j >> 2] |= (unsigned)(unsigned char)w[ch * ld + k0 + j] << (8 * (j & 3));
-    *(u32x4 *)(packed + i * 16) = u32x4{r[0], r[1], r[2], r[3]};
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (long)gridDim.x * 256) {          // one 16-byte lane of a fragment
+        const long frag = i >> 6;
+        const int lane = (int)(i & 63), ch = (int)(frag / kb_total) * 16 + (lane & 15);
+        const int k0 = (int)(frag % kb_total) * 64 + (lane >> 4) * 16;
+        unsigned r[4] = {0, 0, 0, 0};
+        if (ch < n)
+            for (int j = 0; j < 16; ++j)
+                if (k0 + j < k) r[j >> 2] |= (unsigned)(unsigned char)w[ch * ld + k0 + j] << (8 * (j & 3));
+        *(u32x4 *)(packed + i * 16) = u32x4{r[0], r[1], r[2], r[3]};
+    }
 }
 
 // float weights [n][ld] -> fragments + scales: one workgroup per channel
 template <int DT>
-__global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld, int n, int k, int kb_total, char *packed, float *scale) {
+__global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld, int n, int n_pad, int k, int kb_total, char *packed, float *scale) {
     __shared__ unsigned red[4];
-    const int ch = blockIdx.x;                                          // < n_pad
-    const char *wr = w + (long)ch * ld * (DT == Y3_BF16 ? 2 : 4);
-    const int kk = ch < n ? k : 0;
-    unsigned m = 0;
-    for (int k0 = threadIdx.x * 8; k0 < kk; k0 += 256 * 8) {
-        unsigned v[8];
-        Chunk<DT>::load(wr, k0, kk - k0, v);
-        m = amax8(v, m);
+    for (int ch = blockIdx.x; ch < n_pad; ch += gridDim.x) {
+        const char *wr = w + (long)ch * ld * (DT == Y3_BF16 ? 2 : 4);
+        const int kk = ch < n ? k : 0;
+        unsigned m = 0;
+        for (int k0 = threadIdx.x * 8; k0 < kk; k0 += 256 * 8) {
+            unsigned v[8];
+            Chunk<DT>::load(wr, k0, kk - k0, v);
+            m = amax8(v, m);
+        }
+        m = lanes_max<64>(m, [](unsigned a, unsigned b) { return max(a, b); });
+        __syncthreads();                                                // (red has been read)
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = max(max(red[0], red[1]), max(red[2], red[3]));
+        const RowScale r = row_scale(m);
+        for (int k0 = threadIdx.x * 8; k0 < kb_total * 64; k0 += 256 * 8) {
+            unsigned v[8];
+            Chunk<DT>::load(wr, k0, kk - k0, v);
+            unsigned lo = q4(v[0], v[1], v[2], v[3], r.inv), hi = q4(v[4], v[5], v[6], v[7], r.inv);
+            if (!r.finite) lo = hi = 0;
+            const long frag = (long)(ch >> 4) * kb_total + (k0 >> 6);
+            const int lane = (ch & 15) + 16 * ((k0 >> 4) & 3);
+            *(unsigned long long *)(packed + frag * 1024 + lane * 16 + (k0 & 8)) = (unsigned long long)hi << 32 | lo;
+        }
+        if (threadIdx.x == 0 && ch < n) scale[ch] = r.s;
     }
-    m = wave_umax(m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = max(max(red[0], red[1]), max(red[2], red[3]));
-    const RowScale r = row_scale(m);
-    for (int k0 = threadIdx.x * 8; k0 < kb_total * 64; k0 += 256 * 8) {
-        unsigned v[8];
-        Chunk<DT>::load(wr, k0, kk - k0, v);
-        unsigned lo = q4(v[0], v[1], v[2], v[3], r.inv), hi = q4(v[4], v[5], v[6], v[7], r.inv);
-        if (!r.finite) lo = hi = 0;
-        const long frag = (long)(ch >> 4) * kb_total + (k0 >> 6);
-        const int lane = (ch & 15) + 16 * ((k0 >> 4) & 3);
-        *(unsigned long long *)(packed + frag * 1024 + lane * 16 + (k0 & 8)) = (unsigned long long)hi << 32 | lo;
-    }
-    if (threadIdx.x == 0 && ch < n) scale[ch] = r.s;
 }
 
 // ---- the product ------------------------------------------------------------------------------------------------
@@ -902,6 +898,8 @@ int check_desc(const y3_linear_i8_desc *d) {
                "linear_i8: k_pad %d / n_pad %d are not y3_linear_i8_layout's", d->k_pad, d->n_pad);
     Y3_REQUIRE(d->rows >= 0 && d->rows <= (1ll << 40) / d->k_pad, Y3_E_INVALID, "linear_i8: %lld rows", (long long)d->rows);
     Y3_REQUIRE((d->flags & ~Y3_CONV_LEAKY) == 0, Y3_E_INVALID, "linear_i8: flags 0x%x", d->flags);
+    Y3_REQUIRE(d->rows == 0 || (d->x_ld <= (1ll << 44) / d->rows && d->out_ld <= (1ll << 44) / d->rows), Y3_E_INVALID, "linear_i8: %lld rows on x_ld %lld, out_ld %lld",
+               (long long)d->rows, (long long)d->x_ld, (long long)d->out_ld);
     Y3_REQUIRE(d->x_ld >= d->k && d->out_ld >= d->n, Y3_E_INVALID, "linear_i8: x_ld %lld < k or out_ld %lld < n",
                (long long)d->x_ld, (long long)d->out_ld);
     return Y3_OK;
@@ -982,9 +980,9 @@ extern "C" int y3_linear_i8_pack(const y3_linear_i8_desc *d, int w_dtype, const 
     const int kb = d->k_pad / 64;
     if (w_dtype == Y3_I8) {
         const long chunks = (long)d->n_pad / 16 * kb * 64;
-        hipLaunchKernelGGL(pack_i8_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, st, (const char *)w, (long)w_ld, d->n, d->k, kb, chunks, (char *)packed);
-    } else if (w_dtype == Y3_BF16) hipLaunchKernelGGL(pack_float_kernel<Y3_BF16>, dim3(d->n_pad), dim3(256), 0, st, (const char *)w, (long)w_ld, d->n, d->k, kb, (char *)packed, scale);
-    else hipLaunchKernelGGL(pack_float_kernel<Y3_F32>, dim3(d->n_pad), dim3(256), 0, st, (const char *)w, (long)w_ld, d->n, d->k, kb, (char *)packed, scale);
+        hipLaunchKernelGGL(pack_i8_kernel, dim3(rows_grid((chunks + 255) / 256)), dim3(256), 0, st, (const char *)w, (long)w_ld, d->n, d->k, kb, chunks, (char *)packed);
+    } else if (w_dtype == Y3_BF16) hipLaunchKernelGGL(pack_float_kernel<Y3_BF16>, dim3(rows_grid(d->n_pad)), dim3(256), 0, st, (const char *)w, (long)w_ld, d->n, d->n_pad, d->k, kb, (char *)packed, scale);
+    else hipLaunchKernelGGL(pack_float_kernel<Y3_F32>, dim3(rows_grid(d->n_pad)), dim3(256), 0, st, (const char *)w, (long)w_ld, d->n, d->n_pad, d->k, kb, (char *)packed, scale);
     return y3_check_launch("linear_i8_pack");
 }
 

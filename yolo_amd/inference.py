@@ -214,6 +214,9 @@ def run_inference(img_path, output_dir, args):
     shorter).  A batch is B independent batch-1 runs and the batched plan gives an image the same bits
     whatever the batch size, so the files do not depend on N (tests: byte-identical to batch 1 run with --no_splitk;
     batch 1 splits small launches over k by default, which adds the partial sums in another order)."""
+    n_alt = int(getattr(args, "alternatives", 0) or 0)
+    if not 0 <= n_alt <= min(32, config.num_classes):
+        raise ValueError("alternatives: 0 .. %d" % min(32, config.num_classes))
     for d in (output_dir, os.path.join(output_dir, "images"), os.path.join(output_dir, "labels")):
         if not os.path.exists(d):
             os.mkdir(d)
@@ -232,7 +235,6 @@ def run_inference(img_path, output_dir, args):
     output_nodes = yolo(input_images=None, is_training=False, config_path=cfg_path, num_classes=num_classes,
                         dtype=getattr(args, "dtype", None), splitk=batch == 1 and not getattr(args, "no_splitk", False),
                         int8=bool(getattr(args, "int8", False)))
-    n_alt = int(getattr(args, "alternatives", 0) or 0)
     if n_alt:
         os.makedirs(os.path.join(output_dir, "alternatives"), exist_ok=True)
     weights = getattr(args, "weights", None) or config.yolov3_weights_path

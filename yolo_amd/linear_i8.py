@@ -170,8 +170,8 @@ class Int8Linear(object):
             return out
         scale_ptr = None
         if code == _lib.Y3_I8:
-            if scale.dtype != torch.float32 or scale.numel() != rows or scale.device != device:
-                raise ValueError("scale must be float32 with one value per row on %s" % device)
+            if scale.dtype != torch.float32 or scale.device != device or scale.shape not in (x.shape[:-1], (rows,)):
+                raise ValueError("scale must be float32 %r on %s" % (tuple(x.shape[:-1]), device))
             scale = scale.contiguous()
             scale_ptr = scale.data_ptr()
             m, x_ld = _eight_bit_rows(m, self.n)
