@@ -155,6 +155,22 @@ def test_equal_largest_logits(C, top):
         check(log_probs(zc, ic, top=top), z, ids, top)
 
 
+@pytest.mark.parametrize("rows,C,ld", [(34001, 65536, 65536), (30000001, 80, 80), (5, 700, 1 << 30), (5, 5000, 1 << 30)])
+def test_rows_past_32_bits(rows, C, ld):
+    """More than 2^31 logits, of which the first and last rows are looked at."""
+    g = torch.Generator().manual_seed(C)
+    z = torch.zeros(rows * ld, dtype=torch.bfloat16, device="cuda").as_strided((rows, C), (ld, 1))
+    m = min(rows, 50)
+    ends = [(3 * torch.randn(m, C, generator=g)).to(torch.bfloat16) for _ in range(2)]
+    z[:m], z[-m:] = ends[0].cuda(), ends[1].cuda()
+    if rows == m:
+        ends[0] = ends[1]
+    ids = torch.randint(0, C, (rows,), generator=g).int().cuda()
+    got = log_probs(z, ids, top=3)
+    for part, at in ((ends[0], slice(0, m)), (ends[1], slice(rows - m, rows))):
+        check(type(got)(*[v[at] for v in got]), part, ids[at].cpu(), 3)
+
+
 def test_strides():
     g = torch.Generator().manual_seed(1)
     C = 80
@@ -221,6 +237,16 @@ def test_refusals():
                 lambda: log_probs(z.detach(), ids, top=1, out=(f, f, None, None))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_outputs_in_the_logits_are_refused():
+    buf = torch.zeros(40 * 85, device="cuda")
+    z = buf.view(40, 85)[:, :80]
+    good = [torch.empty(40, device="cuda"), torch.empty(40, device="cuda"), None, None]
+    log_probs(z, torch.zeros(40, dtype=torch.int64, device="cuda"), out=tuple(good))
+    good[1] = buf[85 * 39 + 40 - 1:][:40]
+    with pytest.raises(ValueError, match="overlap"):
+        log_probs(z, torch.zeros(40, dtype=torch.int64, device="cuda"), out=tuple(good))
 
 
 @pytest.mark.parametrize("rows,C", [(1, 128000), (16, 40000), (3000, 80)])

@@ -274,6 +274,41 @@ def test_more_rows_than_a_grid():
             assert torch.equal(got[lo:lo + (1 << 24)], part.bfloat16())
 
 
+@pytest.mark.parametrize("rows,k,n,x", [(1200007, 2048, 16, "bf16"), (17500001, 128, 64, "bf16"), (70001, 32768, 16, "bf16"), (9000001, 128, 256, "f32"),
+                                        (540001, 8192, 300, "i8"), (9, 100, 40, "bf16")])
+def test_rows_past_32_bits(rows, k, n, x):
+    """Inputs of more than 4 GB, of which the first and last rows are looked at; few rows on a pitch of 2^30 elements."""
+    rng = np.random.default_rng(k)
+    lay, w, t, b = layer_of(rng, n, k, True, True, "f32")
+    if rows == 9:
+        xs = torch.zeros(9 << 30, dtype=torch.bfloat16, device="cuda").as_strided((9, k), (1 << 30, 1))
+    else:
+        xs = torch.zeros(rows, k, dtype=torch.int8 if x == "i8" else DT[x], device="cuda")
+    m = min(rows, 100)
+    head, tail = torch.from_numpy(rows_of(rng, m, k)), torch.from_numpy(rows_of(rng, m, k))
+    if x == "i8":
+        head, tail = (torch.from_numpy(rng.integers(-128, 128, (m, k)).astype(np.int8)) for _ in range(2))
+    head, tail = head.to(xs.dtype), tail.to(xs.dtype)
+    xs[:m], xs[-m:] = head.cuda(), tail.cuda()
+    if rows == m:
+        head = tail
+    s = torch.full((rows,), 0.5, device="cuda") if x == "i8" else None
+    got = lay(xs, scale=s)
+    for part, y in ((head, got[:m]), (tail, got[-m:])):
+        q, sc = (part.numpy(), np.full(m, 0.5, np.float32)) if x == "i8" else rule(part.float().numpy())
+        close(y, *want(q, sc, w, t, b, True), "f32")
+
+
+def test_tiles_past_32_bits():
+    rows, k, n = 40001, 512, 60001
+    w = torch.randint(-128, 128, (n, k), dtype=torch.int8, device="cuda")
+    x = torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda")
+    got = Int8Linear(w, scale=torch.full((n,), 2.0 ** -6, device="cuda"))(x, scale=torch.ones(rows, device="cuda"))
+    for lo in range(0, rows, 8000):
+        part = x[lo:lo + 8000].float() @ w.float().t() * 2.0 ** -6                           # (integers below 2^24: exact)
+        assert torch.equal(got[lo:lo + 8000], part.bfloat16())
+
+
 @pytest.mark.parametrize("k", [130, 20])
 def test_very_many_channels(k):
     """2^24 channels: weights and outputs past 32-bit offsets."""

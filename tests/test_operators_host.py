@@ -86,6 +86,9 @@ def test_quantize_and_pack_refusals(lib):
     assert pack(0, None, 100, P, P) == -1
 
 
+O = P + (1 << 32)                                       # outputs, far from the logits
+
+
 def probs(**kw):
     d = _lib.LogProbsDesc()
     d.dtype, d.classes, d.rows, d.group, d.group_ld, d.row_ld, d.top, d.extent = _lib.Y3_F32, 80, 10, 1, 85, 0, 3, 9 * 85 + 80
@@ -99,20 +102,27 @@ def probs(**kw):
                                 dict(group=3, group_ld=256, row_ld=85, extent=3 * 256 + 79)])
 def test_log_probs_descriptor_refusals(lib, kw):
     d = probs(**kw)
-    assert lib.y3_log_probs(ctypes.byref(d), P, None, P, P, P, P, P, P, 1 << 40, None) == -1
+    assert lib.y3_log_probs(ctypes.byref(d), P, None, P, O, O, O, O, P, 1 << 40, None) == -1
+    assert b"overlap" not in lib.y3_last_error()
 
 
 def test_log_probs_pointer_refusals(lib):
     d = probs()
     call = lambda *a: lib.y3_log_probs(ctypes.byref(d), *a, P, 1 << 40, None)  # noqa: E731
-    assert call(None, None, P, P, P, P, P) == -1
-    assert call(P, None, None, P, P, P, P) == -1
-    assert call(P, None, P, None, P, P, P) == -1
-    assert call(P, None, P, P, P, None, P) == -1
-    assert call(P + 2, None, P, P, P, P, P) == -2
-    assert call(P, P + 4, P, P, P, P, P) == -2
-    assert call(P, None, P + 2, P, P, P, P) == -2
-    assert call(P, None, P, P, P + 1, P, P) == -2
+    assert call(None, None, P, O, O, O, O) == -1
+    assert call(P, None, None, O, O, O, O) == -1
+    assert call(P, None, P, None, O, O, O) == -1
+    assert call(P, None, P, O, O, None, O) == -1
+    assert call(P + 2, None, P, O, O, O, O) == -2
+    assert call(P, P + 4, P, O, O, O, O) == -2
+    assert call(P, None, P + 2, O, O, O, O) == -2
+    assert call(P, None, P, O + 1, O, O, O) == -2
+    end = P + (9 * 85 + 80) * 4
+    for i, n in enumerate((10, 10, 30, 30)):                         # outputs that reach into the logits
+        for at in (P, end - 4, P - 4 * n + 4, P + 82 * 4):
+            outs = [O] * 4
+            outs[i] = at
+            assert call(P, None, P, *outs) == -1 and b"overlap" in lib.y3_last_error()
     d = probs(rows=0)
     assert call(None, None, None, None, None, None, None) == 0
 

@@ -681,6 +681,7 @@ extern "C" int y3_log_probs(const y3_log_probs_desc *d, const void *logits, cons
     Y3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Y3_E_INVALID, "log_probs: workspace of %lld bytes, needs %lld", (long long)workspace_bytes, (long long)need);
     Y3_REQUIRE((uintptr_t)logits % (d->dtype == Y3_F32 ? 4 : 2) == 0 && (uintptr_t)ids % (d->ids_64 ? 8 : 4) == 0 && (uintptr_t)row_offsets % 8 == 0 &&
                ((uintptr_t)logp | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_logp) % 4 == 0 && aligned16(workspace), Y3_E_ALIGN, "log_probs: pointer not aligned");
+    int64_t span = d->extent;                                    // logits from the first row's first to the last row's last
     if (!row_offsets) {
         Y3_REQUIRE(d->group >= 1 && d->group_ld >= 0 && d->row_ld >= 0 && d->group_ld <= (1ll << 40) && d->row_ld <= (1ll << 40), Y3_E_INVALID,
                    "log_probs: group %d, group_ld %lld, row_ld %lld", d->group, (long long)d->group_ld, (long long)d->row_ld);
@@ -689,7 +690,12 @@ extern "C" int y3_log_probs(const y3_log_probs_desc *d, const void *logits, cons
         const double last = (double)g * d->group_ld + (double)in_last * d->row_ld;
         const double whole = g > 0 ? (double)(g - 1) * d->group_ld + (double)(d->group - 1) * d->row_ld : 0.0;
         Y3_REQUIRE((last > whole ? last : whole) + d->classes <= (double)d->extent, Y3_E_INVALID, "log_probs: %lld rows reach behind the extent of %lld elements", (long long)d->rows, (long long)d->extent);
+        span = (int64_t)(last > whole ? last : whole) + d->classes;
     }
+    const struct { const void *p; int64_t bytes; } outs[4] = {{logp, d->rows * 4}, {entropy, d->rows * 4}, {top_ids, d->rows * d->top * 4}, {top_logp, d->rows * d->top * 4}};
+    for (const auto &o : outs)
+        Y3_REQUIRE(!o.p || !o.bytes || (uintptr_t)o.p + o.bytes <= (uintptr_t)logits || (uintptr_t)logits + span * (d->dtype == Y3_F32 ? 4 : 2) <= (uintptr_t)o.p, Y3_E_INVALID,
+                   "log_probs: an output overlaps the logits");
     ProbsArgs a;
     a.z = (const char *)logits; a.row_offsets = row_offsets; a.ids = ids; a.logp = logp; a.entropy = entropy; a.top_ids = top_ids; a.top_logp = top_logp;
     a.rows = d->rows; a.group_ld = d->group_ld; a.row_ld = d->row_ld; a.extent = d->extent;
