@@ -382,23 +382,26 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     __syncthreads();
     Row row = {0.0f, 0.0f, 0.0f, false};
     if (wave == 0) {
-        if (top) {
+        if (top) {                                               // (the lowest bits left at 0: a bound a little below)
+            constexpr int BOUND_BITS = DT == Y3_F32 ? 8 : 16;
             unsigned t = 0;
             const unsigned o = order_of(quads[lane]);
 #pragma unroll
-            for (int b = 31; b >= 0; --b) {
+            for (int b = 31; b >= BOUND_BITS; --b) {
                 const unsigned more = t | 1u << b;
                 t = __popcll(__ballot(o >= more)) >= top ? more : t;
             }
-            if (lane == 0) bound_s = of_order(t);
+            if (lane == 0) bound_s = of_order(max(t, 0x007fffffu));     // (-inf: below it there are only NaN's patterns)
         }
+    }
+    if (wave == (p.chunks == 1 ? 0 : W - 1)) {                   // (the first wave writes a whole row's alternatives: it needs these)
         s = Sums{part[0][0], part[0][1], part[0][2]};
 #pragma unroll
         for (int w = 1; w < W; ++w) s = join(s, Sums{part[w][0], part[w][1], part[w][2]});
         if (p.chunks == 1) {
             row = finish(s);
             if (tid == 0) put_scalars(p, r, zid, id, row.m, row.log_z, row.entropy);
-        } else if (tid == 0) p.sums[i] = f32x4{s.m, s.z, s.s, 0.0f};
+        } else if (lane == 0) p.sums[i] = f32x4{s.m, s.z, s.s, 0.0f};
     }
     if (top) {
         __syncthreads();
