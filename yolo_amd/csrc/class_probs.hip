@@ -21,7 +21,7 @@ struct ProbsArgs {
     int32_t *top_ids;
     long rows, group_ld, row_ld, extent, first;
     int classes, group, top, ids_64, fast_group, chunks, chunk_vecs, chunk_more;
-    f32x4 *sums;                       // rows of several chunks: {M, Z, S} and `top` keys per chunk
+    f32x4 *sums;                       // rows of several chunks: {M, Z, S, the id's logit or 0} and `top` keys per chunk
     unsigned long long *keys;
     FastDiv fd_group;                  // r / group where fast_group is set (more than one row per group, fewer than 2^31 rows)
 };
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void probs_lanes_kernel(const ProbsArgs p) {
 // candidates for the alternatives.  For those, the top-th largest of the 64 quads' maxima (found by bisection of its bits,
 // one ballot each) is a bound that at least `top` logits reach and few others do: those are listed, and ranked by counting
 // the larger keys.  A list that overflows (hundreds of equal logits at the border) is settled by one search per alternative.
-// Rows of more than one chunk leave {M, Z, S} and the chunk's first `top` keys in the workspace for probs_join_kernel, which
+// Rows of more than one chunk leave {M, Z, S}, the id's logit and the chunk's first `top` keys in the workspace for probs_join_kernel, which
 // merges them in a fixed order.  One workgroup walking a whole row instead: 31 us for one row of 128000 (its exponentials
 // alone keep one CU busy for 9 us), 98 us for 4096 rows of 32001.
 constexpr int LIST = 512, CHUNK_THREADS = 256;
@@ -306,13 +306,13 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
     }
     long id = -1;
     float zid = 0.0f;
-    if (tid == 0) {
-        if (p.logp && p.chunks == 1) {
+    if (tid == (p.chunks == 1 ? 0 : STEP - 64)) {                // (by the wave that writes it; of several chunks the one that has it)
+        if (p.logp) {
             id = row_id(p, r);
-            if (id >= 0 && id < C) zid = logit<DT>(z, id);
+            if (id >= c0 && id < c1) zid = logit<DT>(z, id);
         }
-        list_n = 0;
     }
+    if (tid == 0) list_n = 0;
     if (top) *(u32x4 *)(list + 2 * tid) = u32x4{0, 0, 0, 0};
     const auto value = [&](int g, int j) {
         if constexpr (DT == Y3_F32) return __uint_as_float(raw[g][j]);
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
         if (p.chunks == 1) {
             row = finish(s);
             if (tid == 0) put_scalars(p, r, zid, id, row.m, row.log_z, row.entropy);
-        } else if (lane == 0) p.sums[i] = f32x4{s.m, s.z, s.s, 0.0f};
+        } else if (lane == 0) p.sums[i] = f32x4{s.m, s.z, s.s, zid};
     }
     if (top) {
         __syncthreads();
@@ -492,26 +492,25 @@ __global__ __launch_bounds__(CHUNK_THREADS) void probs_join_kernel(const ProbsAr
                 bound = k > bound ? k : bound;
             }
         Sums s = {-__builtin_inff(), 0.0f, 0.0f};
+        float zid = 0.0f;
         for (int c = lane; c < p.chunks; c += 64) {
             const f32x4 v = p.sums[r * p.chunks + c];
             s = join(s, Sums{v[0], v[1], v[2]});
+            zid += v[3];                                         // (the id's logit in one chunk, 0 in the others)
         }
         constexpr int AHEAD = 4;                                 // keys of this thread, requested before they are needed
         u64 mine[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) mine[j] = tid + j * threads < n_keys ? keys[tid + j * threads] : 0;
         long id = -1;
-        float zid = 0.0f;
         if (tid == 0) {
             list_n = 0;
-            if (p.logp) {
-                id = row_id(p, r);
-                if (id >= 0 && id < p.classes) zid = logit<DT>(p.z + at * (DT == Y3_F32 ? 4 : 2), id);
-            }
+            if (p.logp) id = row_id(p, r);
         }
         if (top)
             for (int q = tid; q < LIST / 2; q += threads) *(u32x4 *)(list + 2 * q) = u32x4{0, 0, 0, 0};
         const Row row = finish(wave_join(s));
+        zid = wave_reduce(zid, 0.0f, Add());
         if (tid == 0) put_scalars(p, r, zid, id, row.m, row.log_z, row.entropy);
         if (top) {
             bound = wave_max_u64(bound);
