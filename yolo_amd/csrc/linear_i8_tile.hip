@@ -74,7 +74,7 @@ void linear_i8_tile_kernel(const LinArgs p, int m_tiles, int n_tiles, int total)
         const long m0 = (long)mt * 256, n0 = (long)nt * 256;
         rs_x = rsrc(p.x + m0 * p.x_ld, (min(p.rows - m0, 256L) - 1) * p.x_ld + p.k16);
         rs_w = rsrc(p.w + nt * 16 * w_tile_bytes, min((p.n + 15) / 16 - nt * 16, 16) * w_tile_bytes);
-        char *vec = smem + TL_VEC + l_par * 3072 + wn * 256;
+        char *vec = smem + TL_VEC + l_par * (3 * 1024) + wn * 256;
         if (wm == 0) {
             bufdma4(rsrc(p.x_scale + m0, (p.rows - m0) * 4), wn * 256 + lane * 4, vec);
             bufdma4(rsrc(p.bias ? p.bias + n0 : p.w_scale, p.bias ? (p.n - n0) * 4 : 0), wn * 256 + lane * 4, vec + 2048);
@@ -211,7 +211,7 @@ void linear_i8_tile_kernel(const LinArgs p, int m_tiles, int n_tiles, int total)
         // ---- epilogue: channels fq 4 .. + 3 of each 16, for rows frow of each 16 ----------------------------------------
         int mt, nt;
         place(c_tile, mt, nt);
-        const char *vec = smem + TL_VEC + c_par * 3072;
+        const char *vec = smem + TL_VEC + c_par * (3 * 1024);
         float s[8];
 #pragma unroll
         for (int mi = 0; mi < 8; ++mi) s[mi] = *(const float *)(vec + (wm * 128 + mi * 16 + frow) * 4);
