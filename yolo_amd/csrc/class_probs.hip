@@ -98,7 +98,7 @@ struct MinI { __device__ __forceinline__ int operator()(int a, int b) const { re
 // so a round is one subtraction and half a v_min3_u32 per logit (finding the maximum and its class and taking it out costs
 // four times as much: 1.1 M rows of 80, three alternatives, 188 us that way).  bf16 keys are exact.  fp32 keys that agree in
 // all but the class leave open which logit is larger: one more round shows whether any of the first `top` + 1 do, and the
-// wave then settles its rows with whole logits.
+// wave then settles its rows with whole logits.  Bound by memory: those 1.1 M rows of 80 fp32 91 us, 4.3 TB/s.
 template <int DT, int L, int E>
 __global__ __launch_bounds__(256) void probs_lanes_kernel(const ProbsArgs p) {
     constexpr int RPW = 64 / L, SURE = E - 2;                    // the first SURE logits of every lane exist (launch_probs)
@@ -195,9 +195,11 @@ __global__ __launch_bounds__(256) void probs_lanes_kernel(const ProbsArgs p) {
 // candidates for the alternatives.  For those, the top-th largest of the 64 quads' maxima (found by bisection of its bits,
 // one ballot each) is a bound that at least `top` logits reach and few others do: those are listed, and ranked by counting
 // the larger keys.  A list that overflows (hundreds of equal logits at the border) is settled by one search per alternative.
-// Rows of more than one chunk leave {M, Z, S}, the id's logit and the chunk's first `top` keys in the workspace for probs_join_kernel, which
-// merges them in a fixed order.  One workgroup walking a whole row instead: 31 us for one row of 128000 (its exponentials
-// alone keep one CU busy for 9 us), 98 us for 4096 rows of 32001.
+// Rows of more than one chunk leave {M, Z, S}, the id's logit and the chunk's first `top` keys in the workspace for
+// probs_join_kernel, which merges them in a fixed order.  One workgroup walking a whole row instead: 31 us for one row of
+// 128000 (its exponentials alone keep one CU busy for 9 us), 98 us for 4096 rows of 32001.
+//   Bound by vector issue (70 % busy): 4096 rows of 32001 bf16, 262 MB, 72 us and 6 for the join; one row of 128000 7 us and
+//   6, all of it latency.
 constexpr int LIST = 512, CHUNK_THREADS = 256;
 
 typedef unsigned long long u64;
@@ -558,8 +560,7 @@ __global__ __launch_bounds__(CHUNK_THREADS) void probs_join_kernel(const ProbsAr
     }
 }
 
-// Rows of more than 1024 classes: equal chunks of at most 32 logits per thread.
-// Whole rounds of the threads, so that only the last chunk has any that are not filled -- unless that one would be left
+// Rows of more than 1024 classes: chunks of at most 32 logits per thread.  Whole rounds of the threads, so that only the last chunk has any that are not filled -- unless that one would be left
 // with few: then all are equal but for one vector (29 rows of 41221, 20 alternatives, 34 vectors left: 33 us against 7).
 struct Chunks { int n, vecs, more; };
 Chunks chunks_of(const y3_log_probs_desc *d) {

@@ -142,7 +142,8 @@ template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(uns
 
 // ---- rows -> 8-bit rows + scales --------------------------------------------------------------------------------
 // TPR threads per row, 256 / TPR rows per workgroup (TPR = 64: a wave each), a thread's NI chunks kept in registers between
-// the maximum and the division; rows of more than 8 TPR NI values are read twice, the second time from cache.
+// the maximum and the division; rows of more than 8 TPR NI values are read twice, the second time from cache.  Bound by
+// memory, or by the latency of one round trip: 24 rows of 8192 bf16 3.5 us.
 template <int DT, int TPR, int NI>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void quant_rows_kernel(const char *x, long x_ld, long rows, int k, char *q, long q_ld, int k_fill, float *scale) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1, WAVES = TPR / 64;
@@ -255,8 +256,13 @@ __global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld,
 // ---- the product ------------------------------------------------------------------------------------------------
 // Panel kernel: a workgroup of eight waves takes 16 RT rows and 16 NT WN channels (WN WK = 8: WN waves side by side along the
 // channels, WK along k).  The rows' 8-bit values are in LDS -- quantised there from float rows, all of k at once, or copied
-// from 8-bit rows in slabs of k -- and every wave reads its weights as whole fragments straight into registers, two
-// groups of eight ahead: weights are used by one wave each, LDS would only add a copy.
+// from 8-bit rows in slabs of k, the next one requested before this one is multiplied -- and every wave reads its weights as
+// whole fragments straight into registers, one k-block ahead (waves along k: four): weights are used by one wave each, LDS
+// would only add a copy.  Waves along k take aligned 8-bit rows as fragments from memory as well.
+//   Bound by: few rows, the weights' way from memory (1 x 4096 -> 4096, 17 MB: 5.0 us); the middle, the latencies of rows,
+//   weights and stores in turn (1777 x 1003 -> 777 fp32 10 us, 7.4 without the products); many rows, the CUs' reads of
+//   weights from L2 and the stores, all workgroups in the same phase (23104 x 1024 -> 512: 24 us, 15.8 without the products,
+//   21.3 without the stores).  Four k-blocks of weights ahead, or 96 and 128 rows at two waves a SIMD: no faster.
 //   LDS: rows on a pitch of 32 bytes more than their length (16 rows on 16 different 16-byte slots), then per row its scale,
 //   per channel its scale and bias; the area of the rows is used again for the sums of the waves along k.
 constexpr int PN_THREADS = 512, PN_WAVES = 8;
@@ -416,7 +422,8 @@ __device__ __forceinline__ void store_block(const LinArgs &p, char *base, int fr
 // launch and one panel's float rows on their way: the next panel is requested as soon as this one is quantised, and arrives
 // under its products and stores.  LDS holds two panels, so that one barrier per panel is enough.  The two waves of a SIMD
 // belong to different workgroups, so that one's quantisation and stores (vector ALU) run beside the other's products; one
-// workgroup of eight waves and 64 rows, all in step, took 37 us for 92416 x 512 -> 256, the panel kernel 38 us.
+// workgroup of eight waves and 64 rows, all in step, took 37 us for 92416 x 512 -> 256, the panel kernel 38 us.  Bound by
+// memory: 92416 x 512 -> 256 bf16 34 us, 4.2 TB/s; x 256 -> 255 fp32 37 us, 3.8 TB/s (rows of 1020 bytes).
 constexpr int RS_THREADS = 256, RS_ROWS = 32;
 
 // FULL: k = 8 LPR CPL and every panel has its rows (the launcher sees to that), so that no load looks at an end.
