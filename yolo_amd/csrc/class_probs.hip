@@ -560,8 +560,9 @@ __global__ __launch_bounds__(CHUNK_THREADS) void probs_join_kernel(const ProbsAr
     }
 }
 
-// Rows of more than 1024 classes: chunks of at most 32 logits per thread.  Whole rounds of the threads, so that only the last chunk has any that are not filled -- unless that one would be left
-// with few: then all are equal but for one vector (29 rows of 41221, 20 alternatives, 34 vectors left: 33 us against 7).
+// Rows of more than 1024 classes: chunks of at most 32 logits per thread.  Whole rounds of the threads, so that only the
+// last chunk has any that are not filled -- unless that one would be left with few: then all are equal but for one vector
+// (29 rows of 41221, 20 alternatives, 34 vectors left: 33 us against 8.8).
 struct Chunks { int n, vecs, more; };
 Chunks chunks_of(const y3_log_probs_desc *d) {
     if (d->classes <= 1024) return Chunks{0, 0, 0};
