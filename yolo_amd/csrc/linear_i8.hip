@@ -850,12 +850,15 @@ template <int XT> int launch_float(const LinArgs &a, const Panel &c, long cus, h
 }
 
 // The largest block of rows and channels (weights are read once per 16 RT rows, rows once per 16 NT WN channels) that does not
-// leave half of the waves without channels and still gives seven CUs in ten a workgroup.  RT, NT (WK), 8-bit rows, us: 512 x
+// leave half of the waves without channels and still gives six CUs in ten a workgroup.  RT, NT (WK), 8-bit rows, us: 512 x
 // 4096 -> 4096: 2, 2 (256 workgroups) 24, 4, 2 (128) 31, 4, 4 (64) 48; 2048 rows: 62, 53, 57.  bfloat16 rows: 361 x 1024 ->
 // 512: 1, 1, 2 (184) 4.1, 1, 1, 4 (368) 4.6; 8266 x 1717 -> 60: 1, 1, 2 11.5, 2, 1 14.7.  But
 //   4, 2 from two workgroups per CU on, where two fit the LDS: 23104 x 512 -> 255 (361) 15.6, 2, 2 13.6; 46208 x 1024 -> 256
 //   29.6, 31.9; 60000 x 1280 -> 256 (its rows fill half of the LDS) 67, 51;
-//   2, 1 from half of the CUs on, as 16 rows are all that is left: 128 x 4096 -> 4096 (128) 15.7, 1, 1, 2 (512) 23.7;
+//   2, 1 from half of the CUs on, as 16 rows are all that is left, with 8-bit rows (which 16 rows do without LDS, a fragment at
+//   a time) from a third on: 128 x 4096 -> 4096 (128) 15.7, 1, 1, 2 (512) 23.7; 731 x 4096 -> 512 (92) 11.7, 20.3; 731 x 6624
+//   -> 352 (69) 25.6, 1, 1, 4 17.4; bfloat16 200 x 1024 -> 2048 (112) 5.8, 1, 1, 2 5.3;
+//   at most 32 k-blocks a wave where they are along k: 731 x 6624 -> 352 8-bit 1, 1, 2 (276) 25.0, 1, 1, 4 17.4;
 //   3, 4 instead of 4, 4 where the fullest CU then has fewer rows (23104 x 1024 -> 512: 96 rows, 24.3, 128, 26.3; 16384: 96,
 //   28.6, 64, 25.7), or where it fits the LDS twice (60000 x 1280 -> 512: 75, 88).
 Panel panel_of(long rows, int n, int kb, int xt, long cus) {
@@ -876,7 +879,8 @@ Panel panel_of(long rows, int n, int kb, int xt, long cus) {
         } else if (kb > panel_fit(bm)) continue;
         best = t;
         const long groups = (n + cols - 1) / cols, all_of = (rows + bm - 1) / bm * groups;
-        if (c.rt == 4 && c.nt == 2 ? all_of < 2 * cus || !twice(4) : all_of < (c.rt == 2 && c.nt == 1 ? cus / 2 : cus * 7 / 10)) continue;
+        if (c.rt == 4 && c.nt == 2 ? all_of < 2 * cus || !twice(4) : all_of < (c.rt == 2 && c.nt == 1 ? xt >= Y3_I8 ? cus / 3 : cus / 2 : cus * 6 / 10)) continue;
+        if (c.wk > 1 && c.wk < 8 && kb > 32 * c.wk) continue;
         if (c.nt == 4 && xt < Y3_I8 && (fullest(48, groups) < fullest(64, groups) || (!twice(4) && twice(3) && all_of >= 2 * cus))) best.rt = 3;
         break;
     }
@@ -891,13 +895,16 @@ int es_of(int dt) { return dt == Y3_F32 ? 4 : dt == Y3_BF16 ? 2 : 1; }
 // 8-bit rows are made in the workspace first.
 //   Up to 16 rows are quantised by every workgroup, and 64K values take one as long as a launch does (16 rows of 4096 -> 4096:
 //   7.3 us against 7.9, of 8192 -> 8192: 26 against 15.6).
+//   One group of channels quantises each row once, 32 or 16 rows to a workgroup: 8000 x 4096 -> 200 24 us against 40, 60000 x
+//   4096 -> 64 119, 192; from 4096 channels on 16 rows are no better than two launches (60000 x 8192 -> 64: 412, 369).
 //   A tile for every CU and two million weights: a pass over the rows is little beside the product, which the tile kernel
 //   computes faster (8192 x 2048 -> 4096: 116 us against 75, 16384 x 1024 -> 2048: 62, 54; fewer weights or tiles, 32768 x
 //   1024 -> 1024: 58, 62, 65536 x 2048 -> 512: 125, 147, 4096 x 2048 -> 2048: 32, 35).
 bool fused(const y3_linear_i8_desc *d) {
-    const int bm = d->rows <= 16 ? 16 : d->rows <= 32 ? 32 : 64;
+    const int bm = d->rows <= 32 ? 32 : 64;
+    if (d->rows <= 16) return d->k_pad / 64 <= panel_fit(16) && d->rows * d->k_pad <= 65536;
+    if (d->n <= 256 && d->k_pad <= 4096) return true;
     if (d->k_pad / 64 > panel_fit(bm)) return false;
-    if (d->rows <= 16) return d->rows * d->k_pad <= 65536;
     const long tiles = (d->rows + 255) / 256 * ((d->n + 255) / 256);
     return tiles < 256 || (long)d->n * d->k_pad < (1l << 21) || d->k_pad < 512;
 }
