@@ -257,12 +257,12 @@ __device__ __forceinline__ int place_in(const u64 *list, int n, u64 k) {
     return rank;
 }
 
-template <int DT>
-__global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8))) void probs_chunk_kernel(const ProbsArgs p) {
-    constexpr int VE = DT == Y3_F32 ? 4 : 8, ES = DT == Y3_F32 ? 4 : 2, NV = 32 / VE, STEP = CHUNK_THREADS, W = STEP / 64;
+template <int DT, int STEP>
+__global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void probs_chunk_kernel(const ProbsArgs p) {
+    constexpr int VE = DT == Y3_F32 ? 4 : 8, ES = DT == Y3_F32 ? 4 : 2, NV = 32 / VE, W = STEP / 64, GROUP = STEP / 64;         // (GROUP lanes: a "quad")
     __shared__ __attribute__((aligned(16))) u64 list[LIST];
     __shared__ u64 red[W];
-    __shared__ float part[W][3], quads[STEP / 4], bound_s;
+    __shared__ float part[W][3], quads[STEP / GROUP], bound_s;
     __shared__ int list_n;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float ninf = -__builtin_inff();
@@ -315,7 +315,9 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
         }
     }
     if (tid == 0) list_n = 0;
-    if (top) *(u32x4 *)(list + 2 * tid) = u32x4{0, 0, 0, 0};
+    if (top)
+#pragma unroll
+        for (int q = tid; q < LIST / 2; q += STEP) *(u32x4 *)(list + 2 * q) = u32x4{0, 0, 0, 0};
     const auto value = [&](int g, int j) {
         if constexpr (DT == Y3_F32) return __uint_as_float(raw[g][j]);
         else return __uint_as_float(j % 2 ? raw[g][j / 2] & 0xffff0000u : raw[g][j / 2] << 16);
@@ -378,9 +380,9 @@ __global__ __launch_bounds__(CHUNK_THREADS) __attribute__((amdgpu_waves_per_eu(8
             }
     }
     s = wave_join(s);
-    const float quad = lanes_reduce<4>(big, Max());
+    const float quad = lanes_reduce<GROUP>(big, Max());
     if (lane == 0) { part[wave][0] = s.m; part[wave][1] = s.z; part[wave][2] = s.s; }
-    if ((lane & 3) == 0) quads[tid >> 2] = quad;
+    if (lane % GROUP == 0) quads[tid / GROUP] = quad;
     __syncthreads();
     Row row = {0.0f, 0.0f, 0.0f, false};
     if (wave == 0) {
@@ -569,7 +571,8 @@ Chunks chunks_of(const y3_log_probs_desc *d) {
     const int ve = d->dtype == Y3_F32 ? 4 : 8, most = CHUNK_THREADS * 32 / ve;
     const int vecs = 1 + (d->classes + ve - 1) / ve;             // (the most an alignment makes of a row)
     const int n = (vecs + most - 1) / most, each = (int)(((vecs + n - 1) / n + CHUNK_THREADS - 1) / CHUNK_THREADS * CHUNK_THREADS);
-    if (n == 1 || vecs - (n - 1) * each >= 2 * CHUNK_THREADS) return Chunks{n, each, 0};
+    if (n == 1) return Chunks{1, vecs, 0};
+    if (vecs - (n - 1) * each >= 2 * CHUNK_THREADS) return Chunks{n, each, 0};
     return Chunks{n, vecs / n, vecs % n};
 }
 
@@ -594,10 +597,15 @@ template <int DT> int launch_probs(const ProbsArgs &a, hipStream_t st) {
     else if (C <= 512) launch_even<DT, 32, 10>(a, st);
     else if (C <= 1024) launch_even<DT, 64, 10>(a, st);
     else {
+        constexpr int VE = DT == Y3_F32 ? 4 : 8;
         ProbsArgs c = a;
         for (c.first = 0; c.first < a.rows * a.chunks; c.first += 1 << 23) {        // (a grid holds fewer than 2^32 threads)
             const long n = a.rows * a.chunks - c.first;
-            hipLaunchKernelGGL(probs_chunk_kernel<DT>, dim3((unsigned)(n < (1 << 23) ? n : 1 << 23)), dim3(CHUNK_THREADS), 0, st, c);
+            const dim3 grid((unsigned)(n < (1 << 23) ? n : 1 << 23));
+            const int vecs = a.chunk_vecs + (a.chunk_more > 0);
+            if (vecs <= 64 * 32 / VE) hipLaunchKernelGGL((probs_chunk_kernel<DT, 64>), grid, dim3(64), 0, st, c);
+            else if (vecs <= 128 * 32 / VE) hipLaunchKernelGGL((probs_chunk_kernel<DT, 128>), grid, dim3(128), 0, st, c);
+            else hipLaunchKernelGGL((probs_chunk_kernel<DT, CHUNK_THREADS>), grid, dim3(CHUNK_THREADS), 0, st, c);
         }
         if (a.chunks == 1) return y3_check_launch("log_probs");
         const int rc = y3_check_launch("log_probs (chunks)");
