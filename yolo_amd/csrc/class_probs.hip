@@ -190,16 +190,18 @@ __global__ __launch_bounds__(256) void probs_lanes_kernel(const ProbsArgs p) {
 }
 
 // ---- many classes: rows in chunks of up to 8192 logits, one workgroup of four waves per chunk ---------------------------
-// A chunk is read once, in 16-byte vectors, into registers (vector 0 of a row is what lies in front of its first 16-byte
-// border, the last one what lies behind the last), and everything is done there: the thread's maximum, its sums, and the
-// candidates for the alternatives.  For those, the top-th largest of the 64 quads' maxima (found by bisection of its bits,
-// one ballot each) is a bound that at least `top` logits reach and few others do: those are listed, and ranked by counting
-// the larger keys.  A list that overflows (hundreds of equal logits at the border) is settled by one search per alternative.
+// A chunk is read once, in 16-byte vectors at whatever address the row starts (the last one moved into place), into
+// registers, and everything is done there: the thread's maximum, its sums, and the candidates for the alternatives.  For
+// those, the top-th largest of 64 groups' maxima (found by bisection of its upper bits, one ballot each) is a bound that at
+// least `top` logits reach and few others do: those are listed, and ranked by counting the larger keys.  A list that
+// overflows (hundreds of equal logits at the border) is settled by one search per alternative.  A row of up to 2048 (4096)
+// logits is one wave's (two waves'): 20000 rows of 2000 bf16 27 us, by four waves 91.
 // Rows of more than one chunk leave {M, Z, S}, the id's logit and the chunk's first `top` keys in the workspace for
 // probs_join_kernel, which merges them in a fixed order.  One workgroup walking a whole row instead: 31 us for one row of
-// 128000 (its exponentials alone keep one CU busy for 9 us), 98 us for 4096 rows of 32001.
-//   Bound by vector issue (70 % busy): 4096 rows of 32001 bf16, 262 MB, 72 us and 6 for the join; one row of 128000 7 us and
-//   6, all of it latency.
+// 128000 (its exponentials alone keep one CU busy for 9 us), 98 us for 4096 rows of 32001; chunks of 4096 or 2048 logits:
+// 75 and 87 us for the latter against 72.
+//   Bound by vector issue (70 % busy) and memory: 4096 rows of 32001 bf16, 262 MB, 67 us with the join's 6; vectors from the
+//   row's first 16-byte border on, its ends one by one: 71.  One row of 128000: 7 us and 6, all of it latency.
 constexpr int LIST = 512, CHUNK_THREADS = 256;
 
 typedef unsigned long long u64;
@@ -259,10 +261,10 @@ __device__ __forceinline__ int place_in(const u64 *list, int n, u64 k) {
 
 template <int DT, int STEP>
 __global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void probs_chunk_kernel(const ProbsArgs p) {
-    constexpr int VE = DT == Y3_F32 ? 4 : 8, ES = DT == Y3_F32 ? 4 : 2, NV = 32 / VE, W = STEP / 64, GROUP = STEP / 64;         // (GROUP lanes: a "quad")
+    constexpr int VE = DT == Y3_F32 ? 4 : 8, ES = DT == Y3_F32 ? 4 : 2, NV = 32 / VE, W = STEP / 64, GROUP = STEP / 64;         // GROUP lanes have one maximum
     __shared__ __attribute__((aligned(16))) u64 list[LIST];
     __shared__ u64 red[W];
-    __shared__ float part[W][3], quads[STEP / GROUP], bound_s;
+    __shared__ float part[W][3], groups[STEP / GROUP], bound_s;
     __shared__ int list_n;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float ninf = -__builtin_inff();
@@ -275,10 +277,10 @@ __global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void 
         return;
     }
     const char *z = p.z + at * ES;
-    const int C = p.classes, top = p.top, head = (int)((16 - ((uintptr_t)z & 15)) & 15) / ES;
-    const int whole = 1 + (C - head) / VE, v0 = chunk * p.chunk_vecs + min(chunk, p.chunk_more), vecs = p.chunk_vecs + (chunk < p.chunk_more);   // (C > 1024)
-    const int c0 = max(0, head + (v0 - 1) * VE), c1 = min(C, head + (v0 + vecs - 1) * VE);           // the chunk's classes
-    const auto first_of = [&](int g) { return head + (v0 + tid + g * STEP - 1) * VE; };
+    const int C = p.classes, top = p.top, whole = C / VE;
+    const int v0 = chunk * p.chunk_vecs + min(chunk, p.chunk_more), vecs = p.chunk_vecs + (chunk < p.chunk_more);
+    const int c0 = v0 * VE, c1 = min(C, (v0 + vecs) * VE);       // the chunk's classes
+    const auto first_of = [&](int g) { return (v0 + tid + g * STEP) * VE; };
     // What a chunk does not fill holds -1e38: its exponential is 0 beside any logit above -1e37, and no NaN comes of it.
     constexpr unsigned FILL = DT == Y3_F32 ? 0xfe960000u : 0xfe96fe96u;
     u32x4 raw[NV];
@@ -286,22 +288,22 @@ __global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void 
     for (int g = 0; g < NV; ++g) {
         raw[g] = u32x4{FILL, FILL, FILL, FILL};
         const int w0 = wave * 64 + g * STEP;                     // (wave-uniform: all 64 vectors are there and whole)
-        if (v0 + w0 >= 1 && w0 + 63 < vecs && v0 + w0 + 63 < whole) {
-            raw[g] = *(const u32x4 *)(z + (long)(head + (v0 + w0 - 1) * VE) * ES + lane * 16);
-        } else if (w0 < vecs && v0 + w0 <= whole) {
-            const int in = tid + g * STEP, u = v0 + in, b = first_of(g);
-            if (in < vecs) {
-                if (u >= 1 && u < whole) raw[g] = *(const u32x4 *)(z + (unsigned)(b * ES));
-                else if (u <= whole) {
-#pragma unroll 1
-                    for (int j = 0; j < VE; ++j) {               // the vector at an end of the row
-                        if (b + j < 0 || b + j >= C) continue;
-                        const unsigned bits = DT == Y3_F32 ? ((const unsigned *)z)[b + j] : ((const unsigned short *)z)[b + j];
-                        const int word = j * ES / 4, shift = j * ES % 4 * 8;
-                        const unsigned mask = (DT == Y3_F32 ? ~0u : 0xffffu) << shift;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) raw[g][w] = w == word ? (raw[g][w] & ~mask) | bits << shift : raw[g][w];
+        if (w0 + 63 < vecs && v0 + w0 + 63 < whole) __builtin_memcpy(&raw[g], z + (long)(v0 + w0) * 16 + lane * 16, 16);
+        else if (w0 < vecs && v0 + w0 <= whole) {
+            const int u = v0 + tid + g * STEP;
+            if (tid + g * STEP < vecs && u <= whole && u * VE < C) {
+                __builtin_memcpy(&raw[g], z + (long)min(u * VE, C - VE) * ES, 16);
+                if (u == whole) {                                // the row's last logits, moved to the front
+                    const int drop = (VE - (C - whole * VE)) * ES;
+                    u64 lo = (u64)raw[g][1] << 32 | raw[g][0], hi = (u64)raw[g][3] << 32 | raw[g][2];
+                    const u64 fill = (u64)FILL << 32 | FILL;
+                    if (drop >= 8) { lo = hi; hi = fill; }
+                    const int bits = drop % 8 * 8;
+                    if (bits) {
+                        lo = lo >> bits | hi << (64 - bits);
+                        hi = hi >> bits | fill << (64 - bits);
                     }
+                    raw[g] = u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
                 }
             }
         }
@@ -380,16 +382,16 @@ __global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void 
             }
     }
     s = wave_join(s);
-    const float quad = lanes_reduce<GROUP>(big, Max());
+    const float group = lanes_reduce<GROUP>(big, Max());
     if (lane == 0) { part[wave][0] = s.m; part[wave][1] = s.z; part[wave][2] = s.s; }
-    if (lane % GROUP == 0) quads[tid / GROUP] = quad;
+    if (lane % GROUP == 0) groups[tid / GROUP] = group;
     __syncthreads();
     Row row = {0.0f, 0.0f, 0.0f, false};
     if (wave == 0) {
         if (top) {                                               // (the lowest bits left at 0: a bound a little below)
             constexpr int BOUND_BITS = DT == Y3_F32 ? 8 : 16;
             unsigned t = 0;
-            const unsigned o = order_of(quads[lane]);
+            const unsigned o = order_of(groups[lane]);
 #pragma unroll
             for (int b = 31; b >= BOUND_BITS; --b) {
                 const unsigned more = t | 1u << b;
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void 
         const float bound = bound_s;
         if (bound < -1e37f) {
             // from memory, where nothing is filled up; of impossible classes the chunk's first are enough (that is when
-            // fewer than `top` quads have a possible one)
+            // fewer than `top` groups have a possible one)
             for (int c = c0 + tid; c < c1; c += STEP) {
                 const float x = logit<DT>(z, c);
                 if (x >= bound && (x != ninf || c < c0 + top)) {
@@ -569,7 +571,7 @@ struct Chunks { int n, vecs, more; };
 Chunks chunks_of(const y3_log_probs_desc *d) {
     if (d->classes <= 1024) return Chunks{0, 0, 0};
     const int ve = d->dtype == Y3_F32 ? 4 : 8, most = CHUNK_THREADS * 32 / ve;
-    const int vecs = 1 + (d->classes + ve - 1) / ve;             // (the most an alignment makes of a row)
+    const int vecs = (d->classes + ve - 1) / ve;
     const int n = (vecs + most - 1) / most, each = (int)(((vecs + n - 1) / n + CHUNK_THREADS - 1) / CHUNK_THREADS * CHUNK_THREADS);
     if (n == 1) return Chunks{1, vecs, 0};
     if (vecs - (n - 1) * each >= 2 * CHUNK_THREADS) return Chunks{n, each, 0};
