@@ -73,7 +73,7 @@ def test_sizes(C, dt):
 
 
 @pytest.mark.parametrize("rows,C,top", [(1, 80, 3), (2, 50000, 32), (64, 32000, 5), (300, 6000, 1), (1000, 1500, 8), (5000, 80, 5),
-                                        (3, 130001, 20)])
+                                        (3, 130001, 20), (700, 257, 32), (700, 520, 31), (700, 1023, 20)])
 def test_rows(rows, C, top):
     g = torch.Generator().manual_seed(rows)
     z = 4 * torch.randn(rows, C, generator=g)
@@ -82,7 +82,7 @@ def test_rows(rows, C, top):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
-@pytest.mark.parametrize("C", [5, 80, 700, 3000, 40000])
+@pytest.mark.parametrize("C", [5, 80, 300, 700, 1024, 1500, 3000, 6000, 40000])
 def test_hard_rows(C, dt):
     """Ties, masks of -inf and of the type's lowest value, rows that a mask leaves empty, NaN and infinities, large offsets,
     one class far above the rest, all mass in one lane's stretch, rising and falling rows."""

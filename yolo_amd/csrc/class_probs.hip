@@ -564,12 +564,19 @@ __global__ __launch_bounds__(CHUNK_THREADS) void probs_join_kernel(const ProbsAr
     }
 }
 
-// Rows of more than 1024 classes: chunks of at most 32 logits per thread.  Whole rounds of the threads, so that only the
+// Chunks of at most 32 logits per thread.  Whole rounds of the threads, so that only the
 // last chunk has any that are not filled -- unless that one would be left with few: then all are equal but for one vector
 // (29 rows of 41221, 20 alternatives, 34 vectors left: 33 us against 8.8).
+// Up to 1024 classes are the lanes kernel's, but for many alternatives of many classes, whose rounds cost more than a list
+// (20000 rows of 1000 fp32: 5 alternatives 23 us against 25, 20: 54, 31; of 500: 10: 21, 24, 32: 54, 32; 777 bf16: 10: 23,
+// 25, 32: 46, 32), where every lane has a vector.
 struct Chunks { int n, vecs, more; };
+bool in_lanes(const y3_log_probs_desc *d) {
+    const bool f32 = d->dtype == Y3_F32;
+    return d->classes <= (f32 ? 256 : 512) || (d->classes <= 1024 && d->classes * d->top <= (f32 ? 6400 : 9000));
+}
 Chunks chunks_of(const y3_log_probs_desc *d) {
-    if (d->classes <= 1024) return Chunks{0, 0, 0};
+    if (in_lanes(d)) return Chunks{0, 0, 0};
     const int ve = d->dtype == Y3_F32 ? 4 : 8, most = CHUNK_THREADS * 32 / ve;
     const int vecs = (d->classes + ve - 1) / ve;
     const int n = (vecs + most - 1) / most, each = (int)(((vecs + n - 1) / n + CHUNK_THREADS - 1) / CHUNK_THREADS * CHUNK_THREADS);
@@ -594,10 +601,10 @@ template <int DT, int L, int E> void launch_even(const ProbsArgs &a, hipStream_t
 }
 template <int DT> int launch_probs(const ProbsArgs &a, hipStream_t st) {
     const int C = a.classes;
-    if (C <= 128) launch_even<DT, 8, 2>(a, st);
-    else if (C <= 256) launch_even<DT, 16, 10>(a, st);
-    else if (C <= 512) launch_even<DT, 32, 10>(a, st);
-    else if (C <= 1024) launch_even<DT, 64, 10>(a, st);
+    if (a.chunks == 0 && C <= 128) launch_even<DT, 8, 2>(a, st);
+    else if (a.chunks == 0 && C <= 256) launch_even<DT, 16, 10>(a, st);
+    else if (a.chunks == 0 && C <= 512) launch_even<DT, 32, 10>(a, st);
+    else if (a.chunks == 0) launch_even<DT, 64, 10>(a, st);
     else {
         constexpr int VE = DT == Y3_F32 ? 4 : 8;
         ProbsArgs c = a;
