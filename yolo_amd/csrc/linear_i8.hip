@@ -418,17 +418,20 @@ __device__ __forceinline__ void store_block(const LinArgs &p, char *base, int fr
 }
 
 // Resident kernel: few enough weights for the registers of a workgroup (k up to 64 KB, channels up to 64 NT), many rows.
-// Two workgroups of four waves per CU walk panels of 32 rows; a wave keeps the weights of its 16 NT channels for the whole
-// launch and one panel's float rows on their way: the next panel is requested as soon as this one is quantised, and arrives
-// under its products and stores.  LDS holds two panels, so that one barrier per panel is enough.  The two waves of a SIMD
+// Workgroups of four waves, two to four per CU, walk panels of 32 rows; a wave keeps the weights of its 16 NT channels for
+// the whole launch and one panel's float rows on their way: the next panel is requested as soon as this one is quantised, and arrives
+// under its products and stores.  LDS holds two panels, so that one barrier per panel is enough.  The waves of a SIMD
 // belong to different workgroups, so that one's quantisation and stores (vector ALU) run beside the other's products; one
 // workgroup of eight waves and 64 rows, all in step, took 37 us for 92416 x 512 -> 256, the panel kernel 38 us.  Bound by
 // memory: 92416 x 512 -> 256 bf16 34 us, 4.2 TB/s; x 256 -> 255 fp32 37 us, 3.8 TB/s (rows of 1020 bytes).
 constexpr int RS_THREADS = 256, RS_ROWS = 32;
 
+// Workgroups per CU: what the registers allow for up to 128 channels (100000 x 100 -> 64 11.7 us, with two 15.9; 1478656 x 128
+// -> 64 107, 119), two for more (92416 x 256 -> 255 fp32 37, with three 40: more rows written at a time).
+constexpr int rs_per_cu(int xt, int kb, int nt) { return nt == 4 || kb > 8 || (xt == Y3_F32 && kb > 4) ? 2 : kb > 4 ? 3 : 4; }
 // FULL: k = 8 LPR CPL and every panel has its rows (the launcher sees to that), so that no load looks at an end.
 template <int XT, int LPR, int CPL, int KB, int NT, bool FULL, bool F32>
-__global__ __launch_bounds__(RS_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(RS_THREADS) __attribute__((amdgpu_waves_per_eu(rs_per_cu(XT, KB, NT), rs_per_cu(XT, KB, NT))))
 void linear_i8_resident_kernel(const LinArgs p, int panels) {
     constexpr int BM = RS_ROWS, RT = 2, PITCH = KB * 64 + 32, PANEL = BM * PITCH;
     typedef FloatRows<XT, RS_THREADS / 64, BM, LPR, CPL, 1024> Rows;
@@ -825,8 +828,8 @@ int launch_resident_as(const LinArgs &a, long cus, hipStream_t st) {
         }
         attr_dev = dev;
     }
-    const long panels = (a.rows + RS_ROWS - 1) / RS_ROWS;
-    hipLaunchKernelGGL((linear_i8_resident_kernel<XT, LPR, CPL, KB, NT, FULL, F32>), dim3((unsigned)(panels < 2 * cus ? panels : 2 * cus)), dim3(RS_THREADS), lds, st, a, (int)panels);
+    const long panels = (a.rows + RS_ROWS - 1) / RS_ROWS, most = rs_per_cu(XT, KB, NT) * cus, groups = panels < 2 * most ? 2 * cus : most;
+    hipLaunchKernelGGL((linear_i8_resident_kernel<XT, LPR, CPL, KB, NT, FULL, F32>), dim3((unsigned)(panels < groups ? panels : groups)), dim3(RS_THREADS), lds, st, a, (int)panels);
     return y3_check_launch("linear_i8 (resident)");
 }
 // Two panels per workgroup at least, and all channels and k in its registers.
