@@ -970,7 +970,7 @@ extern "C" int y3_quantize_rows_i8(int dtype, const void *x, int64_t rows, int k
     Y3_REQUIRE(dtype == Y3_F32 || dtype == Y3_BF16 || dtype == Y3_I8, Y3_E_INVALID, "quantize_rows_i8: dtype %d", dtype);
     Y3_REQUIRE(k >= 1 && k <= MAX_K, Y3_E_INVALID, "quantize_rows_i8: k = %d outside 1 .. %d", k, MAX_K);
     Y3_REQUIRE(rows >= 0 && rows <= (1ll << 40) / k, Y3_E_INVALID, "quantize_rows_i8: %lld rows", (long long)rows);
-    Y3_REQUIRE(x_ld >= k, Y3_E_INVALID, "quantize_rows_i8: x_ld %lld < k", (long long)x_ld);
+    Y3_REQUIRE(x_ld >= k && (rows == 0 || (x_ld <= (1ll << 44) / rows && q_ld <= (1ll << 44) / rows)), Y3_E_INVALID, "quantize_rows_i8: k %d, x_ld %lld, q_ld %lld", k, (long long)x_ld, (long long)q_ld);
     Y3_REQUIRE(q_ld >= round_up(k, 16) && q_ld % 16 == 0, Y3_E_ALIGN, "quantize_rows_i8: q_ld %lld must be a multiple of 16 that holds k", (long long)q_ld);
     if (rows == 0) return Y3_OK;
     Y3_REQUIRE(x && q && (scale || dtype == Y3_I8), Y3_E_INVALID, "quantize_rows_i8: null pointer");
