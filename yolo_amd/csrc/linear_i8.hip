@@ -392,15 +392,23 @@ __device__ __forceinline__ void store_block(const LinArgs &p, char *base, int fr
             for (int j = 0; j < 4; ++j) y[i][j] = leaky_max(fmaf((float)acc[r][i][j] * t[i][j], sr, b[i][j]), p.slope);
         if (r * 16 + frow >= rows) continue;                     // (lanes that trade places in a swap share their row)
         char *o = base + (unsigned)(r * 16) * row_bytes;
-        if (channels < 16 * NT) {
+        if (channels < 16 * NT) {                                // whole quads in one piece, the last one's channels one by one
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int i = 0; i < NT; ++i) {
+                const int left = channels - i * 16 - fq * 4;
+                char *q = o + (lane_row + (unsigned)(i * 16 + fq * 4) * ES);
+                if (left >= 4) {
+                    if constexpr (F32) *(f32x4_u4 *)q = y[i];
+                    else *(u64_u2 *)q = (unsigned long long)pack_bf16x2(y[i][2], y[i][3]) << 32 | pack_bf16x2(y[i][0], y[i][1]);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i * 16 + fq * 4 + j < channels) {
-                        if constexpr (F32) *(float *)(o + lane_row + (unsigned)(i * 16 + fq * 4 + j) * ES) = y[i][j];
-                        else *(unsigned short *)(o + lane_row + (unsigned)(i * 16 + fq * 4 + j) * ES) = f32_to_bf16(y[i][j]);
-                    }
+                    for (int j = 0; j < 3; ++j)
+                        if (j < left) {
+                            if constexpr (F32) ((float *)q)[j] = y[i][j];
+                            else ((unsigned short *)q)[j] = f32_to_bf16(y[i][j]);
+                        }
+                }
+            }
         } else if constexpr (F32) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) *(f32x4_u4 *)(o + (lane_row + fq * 16u) + i * 64) = y[i];
