@@ -121,7 +121,8 @@ def test_product(rows, k, n, x, out):
 @pytest.mark.parametrize("rows,k,n,x,out", [(33000, 512, 256, "bf16", "bf16"), (32769, 256, 255, "bf16", "f32"), (40000, 128, 128, "bf16", "bf16"),
                                             (32768, 300, 200, "f32", "bf16"), (50001, 100, 64, "f32", "f32"), (33001, 768, 128, "bf16", "bf16"),
                                             (35000, 650, 77, "bf16", "f32"), (33333, 384, 128, "bf16", "bf16"), (32800, 511, 129, "f32", "f32"),
-                                            (60000, 64, 255, "bf16", "bf16"), (34000, 768, 250, "bf16", "bf16")])
+                                            (60000, 64, 255, "bf16", "bf16"), (34000, 768, 250, "bf16", "bf16"), (33007, 256, 255, "f32", "f32"),
+                                            (33005, 500, 129, "bf16", "bf16"), (32801, 128, 1, "bf16", "f32"), (33003, 40, 3, "f32", "bf16")])
 def test_product_of_very_many_rows(rows, k, n, x, out):
     """Panels of rows under weights that stay where they are; wide rows, ragged last panels, odd channels."""
     rng = np.random.default_rng(rows)

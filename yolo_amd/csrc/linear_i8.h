@@ -20,6 +20,7 @@ struct LinArgs {
     int k, k16, n, kb;                 // k rounded up to 16 (bytes of an 8-bit row that may be read), channels, 64-deep k-blocks
     float slope;                       // of the leaky-ReLU; 1: none
     int out_f32;
+    int flat;                          // resident kernel: output rows end to end that do not start on 16 bytes
     int n_groups, slab;                // panel kernel: workgroups along n, k-blocks of a slab
     FastDiv fd_items;
 };

@@ -431,11 +431,12 @@ __device__ __forceinline__ void store_block(const LinArgs &p, char *base, int fr
 // under its products and stores.  LDS holds two panels, so that one barrier per panel is enough.  The waves of a SIMD
 // belong to different workgroups, so that one's quantisation and stores (vector ALU) run beside the other's products; one
 // workgroup of eight waves and 64 rows, all in step, took 37 us for 92416 x 512 -> 256, the panel kernel 38 us.  Bound by
-// memory: 92416 x 512 -> 256 bf16 34 us, 4.2 TB/s; x 256 -> 255 fp32 37 us, 3.8 TB/s (rows of 1020 bytes).
+// memory: 92416 x 512 -> 256 bf16 34 us, 4.2 TB/s.  Output rows that lie end to end but not on 16 bytes are put together in
+// LDS (92416 x 256 -> 255 fp32 32 us, stored quad by quad 39; bf16 27, 35; rows on 16 bytes: 256 bf16 39 that way, 26).
 constexpr int RS_THREADS = 256, RS_ROWS = 32;
 
 // Workgroups per CU: what the registers allow for up to 128 channels (100000 x 100 -> 64 11.7 us, with two 15.9; 1478656 x 128
-// -> 64 107, 119), two for more (92416 x 256 -> 255 fp32 37, with three 40: more rows written at a time).
+// -> 64 107, 119), two for more (92416 x 256 -> 256 fp32 with three 8 % slower: more rows written at a time).
 constexpr int rs_per_cu(int xt, int kb, int nt) { return nt == 4 || kb > 8 || (xt == Y3_F32 && kb > 4) ? 2 : kb > 4 ? 3 : 4; }
 // FULL: k = 8 LPR CPL and every panel has its rows (the launcher sees to that), so that no load looks at an end.
 template <int XT, int LPR, int CPL, int KB, int NT, bool FULL, bool F32>
@@ -510,6 +511,37 @@ void linear_i8_resident_kernel(const LinArgs p, int panels) {
             if (panel + 2 * step < panels) request(panel + 2 * step);
         }
         const long m0 = (long)panel * BM;
+        if (p.flat) {                                            // rows end to end: by way of LDS, stored in whole lines
+            constexpr int ES = F32 ? 4 : 2;
+            char *ob = (char *)(col_b + RS_THREADS / 4 * NT), *o = p.out + m0 * p.out_ld * ES;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int ch = n0 + i * 16 + fq * 4;
+                const f32x4 t = *(const f32x4 *)(col_t + ch), b = *(const f32x4 *)(col_b + ch);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float y = leaky_max(fmaf((float)acc[r][i][j] * t[j], s[r], b[j]), p.slope);
+                        char *at = ob + ((r * 16 + frow) * p.n + ch + j) * ES;
+                        if (ch + j >= p.n) continue;
+                        if constexpr (F32) *(float *)at = y;
+                        else *(unsigned short *)at = f32_to_bf16(y);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            const int whole = nr * p.n * ES / 16;
+            for (int c = tid; c < whole; c += RS_THREADS) *(u32x4 *)(o + c * 16) = *(const u32x4 *)(ob + c * 16);
+            for (int e = whole * 16 / ES + tid; e < nr * p.n; e += RS_THREADS) {
+                if constexpr (F32) ((float *)o)[e] = ((const float *)ob)[e];
+                else ((unsigned short *)o)[e] = ((const unsigned short *)ob)[e];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            continue;
+        }
 #pragma unroll
         for (int i0 = 0; i0 < NT; i0 += 2) {                     // two blocks of channels at a time: registers
             f32x4 t[2], b[2];
@@ -825,13 +857,14 @@ template <int XT> int launch_panel(const LinArgs &a, const Panel &c, hipStream_t
 
 template <int XT, int LPR, int CPL, int KB, int NT, bool FULL, bool F32>
 int launch_resident_as(const LinArgs &a, long cus, hipStream_t st) {
-    constexpr int lds = 2 * RS_ROWS * (KB * 64 + 32) + 2 * RS_ROWS * 4 + 2 * (RS_THREADS / 4 * NT) * 4;
+    constexpr int ES = F32 ? 4 : 2, lds_most = 2 * RS_ROWS * (KB * 64 + 32) + 2 * RS_ROWS * 4 + 2 * (RS_THREADS / 4 * NT) * 4 + RS_ROWS * RS_THREADS / 4 * NT * ES;
+    const int lds = lds_most - (a.flat ? 0 : RS_ROWS * RS_THREADS / 4 * NT * ES);
     static thread_local int attr_dev = -1;
     int dev = 0;
     (void)hipGetDevice(&dev);
     if (attr_dev != dev) {
-        if (hipFuncSetAttribute((const void *)linear_i8_resident_kernel<XT, LPR, CPL, KB, NT, FULL, F32>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
-            y3_set_error("linear_i8: cannot reserve %d bytes of LDS", lds);
+        if (hipFuncSetAttribute((const void *)linear_i8_resident_kernel<XT, LPR, CPL, KB, NT, FULL, F32>, hipFuncAttributeMaxDynamicSharedMemorySize, lds_most) != hipSuccess) {
+            y3_set_error("linear_i8: cannot reserve %d bytes of LDS", lds_most);
             return Y3_E_LAUNCH;
         }
         attr_dev = dev;
@@ -1059,6 +1092,7 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     a.w = (const char *)w; a.w_scale = w_scale; a.bias = bias; a.out = (char *)out;
     a.rows = d->rows; a.out_ld = d->out_ld; a.n = d->n; a.k = d->k; a.kb = d->k_pad / 64;
     a.slope = d->flags & Y3_CONV_LEAKY ? 0.1f : 1.0f; a.out_f32 = d->out_dtype == Y3_F32;
+    a.flat = d->out_ld == d->n && (long)d->n * os % 16 != 0 && aligned16(out);
     if (d->dtype != Y3_I8 && need == 0) {
         const Panel c = panel_of(d->rows, d->n, a.kb, d->dtype, cus);
         return d->dtype == Y3_BF16 ? launch_float<Y3_BF16>(a, c, cus, st) : launch_float<Y3_F32>(a, c, cus, st);
