@@ -438,7 +438,7 @@ constexpr int RS_THREADS = 256, RS_ROWS = 32;
 // Workgroups per CU: what the registers allow for up to 128 channels (100000 x 100 -> 64 11.7 us, with two 15.9; 1478656 x 128
 // -> 64 107, 119), two for more (92416 x 256 -> 256 fp32 with three 8 % slower: more rows written at a time).
 constexpr int rs_per_cu(int xt, int kb, int nt) { return nt == 4 || kb > 8 || (xt == Y3_F32 && kb > 4) ? 2 : kb > 4 ? 3 : 4; }
-// FULL: k = 8 LPR CPL and every panel has its rows (the launcher sees to that), so that no load looks at an end.
+// FULL: k = 8 LPR CPL and every panel has its rows (the launcher sees to that), so that no load looks at an end; not `flat`.
 template <int XT, int LPR, int CPL, int KB, int NT, bool FULL, bool F32>
 __global__ __launch_bounds__(RS_THREADS) __attribute__((amdgpu_waves_per_eu(rs_per_cu(XT, KB, NT), rs_per_cu(XT, KB, NT))))
 void linear_i8_resident_kernel(const LinArgs p, int panels) {
@@ -511,7 +511,7 @@ void linear_i8_resident_kernel(const LinArgs p, int panels) {
             if (panel + 2 * step < panels) request(panel + 2 * step);
         }
         const long m0 = (long)panel * BM;
-        if (p.flat) {                                            // rows end to end: by way of LDS, stored in whole lines
+        if (!FULL && p.flat) {                                   // rows end to end: by way of LDS, stored in whole lines
             constexpr int ES = F32 ? 4 : 2;
             char *ob = (char *)(col_b + RS_THREADS / 4 * NT), *o = p.out + m0 * p.out_ld * ES;
 #pragma unroll
@@ -878,7 +878,7 @@ template <int XT> bool resident_ok(const LinArgs &a, long cus) {
     return a.rows >= 2 * 2 * RS_ROWS * cus && a.rows <= RS_ROWS * 0x3fffffffl && a.n <= 256 && a.out_ld < (1 << 23) && a.kb <= (XT == Y3_BF16 && a.n <= 128 ? 12 : 8);
 }
 template <int XT, int NT, bool F32> int launch_resident(const LinArgs &a, long cus, hipStream_t st) {
-    const bool whole = a.rows % RS_ROWS == 0;
+    const bool whole = a.rows % RS_ROWS == 0 && !a.flat;
     if (a.kb <= 2) return whole && a.k == 128 ? launch_resident_as<XT, 16, 1, 2, NT, true, F32>(a, cus, st) : launch_resident_as<XT, 16, 1, 2, NT, false, F32>(a, cus, st);
     if (a.kb <= 4) return whole && a.k == 256 ? launch_resident_as<XT, 32, 1, 4, NT, true, F32>(a, cus, st) : launch_resident_as<XT, 32, 1, 4, NT, false, F32>(a, cus, st);
     if constexpr (XT == Y3_BF16 && NT == 2)
