@@ -140,7 +140,8 @@ def test_product_of_very_many_rows(rows, k, n, x, out):
     assert torch.equal(lay(xs.cuda()[rows - 70:]), got[rows - 70:])
 
 
-@pytest.mark.parametrize("rows,k,n", [(10001, 200, 520), (16500, 700, 3001), (9003, 120, 1000), (5000, 130, 1500), (3700, 2300, 1040), (10100, 600, 300), (500, 500, 2000), (731, 6624, 352), (200, 6600, 352), (731, 4096, 500), (5690, 2704, 48),
+@pytest.mark.parametrize("rows,k,n", [(10001, 200, 520), (16500, 700, 3001), (9003, 120, 1000), (5000, 130, 1500), (3700, 2300, 1040), (10100, 600, 300),
+                                     (500, 500, 2000), (731, 6624, 352), (200, 6600, 352), (731, 4096, 500), (5690, 2704, 48),
                                      (1700, 3669, 176), (700, 3000, 256), (300, 9000, 30),
                                      (130, 2600, 4000), (6000, 400, 200)])
 @pytest.mark.parametrize("x,out", [("bf16", "bf16"), ("i8", "f32"), ("f32", "f32")])
