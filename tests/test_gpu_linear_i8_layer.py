@@ -1,0 +1,82 @@
+"""-m gpu: a layer of the 8-bit product as an object: when its weights are there, and what may change about it later."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import darknet as od
+from yolo_amd import build_model, config
+from yolo_amd import darknet_weights as dw
+from yolo_amd.linear_i8 import Int8Linear
+
+pytestmark = pytest.mark.gpu
+
+
+def _busy(n=40):
+    """Work queued on the current stream: the launches behind it start milliseconds later."""
+    a = torch.zeros(4096, 4096, device="cuda")
+    b = torch.empty_like(a)
+    for _ in range(n):
+        torch.mm(a, a, out=b)
+
+
+@pytest.mark.parametrize("weights", ["f32", "i8", "cpu"])
+def test_a_layer_made_behind_queued_work_is_called_on_another_stream(weights):
+    n, k = 256, 640
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(300, k, generator=g).to(torch.bfloat16).cuda()
+    w = torch.randint(-127, 128, (n, k), generator=g).to(torch.int8) if weights == "i8" else torch.randn(n, k, generator=g)
+    kw = dict(scale=torch.rand(n, generator=g).cuda()) if weights == "i8" else {}
+    w = w if weights == "cpu" else w.cuda()
+    bias = torch.ones(n, device="cuda")                      # (copies from the host would wait for the queue)
+    ref = Int8Linear(w, bias=bias, **kw)(x)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(one):
+        for size in (n * k, 4 * n):                          # what the layer's allocations would otherwise find
+            for dirt in [torch.full((size,), 101, dtype=torch.uint8, device="cuda") for _ in range(4)]:
+                del dirt
+        _busy()
+        lay = Int8Linear(w, bias=bias, **kw)
+    with torch.cuda.stream(two):
+        got = lay(x)
+    torch.cuda.synchronize()
+    assert torch.equal(got, ref)
+
+
+def test_a_network_packs_on_one_stream_and_runs_on_another():
+    """The 1x1 weights are packed while the first plan is built and serve every later plan."""
+    cfg = config.yolov3_tiny_cfg_path
+    params = dw.random_params(od.parse_layers(cfg, 80)[0], seed=4)
+    x = torch.rand(3, 160, 160, 3, device="cuda")
+    nets = []
+    for _ in range(2):
+        net = build_model.Network(cfg, 80, dtype="bf16", int8=True)
+        net.set_params(params)
+        nets.append(net)
+    ref = [h.clone() for h in nets[0](x)]
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(one):
+        _busy()
+        first = nets[1](x[:1])
+    with torch.cuda.stream(two):
+        got = nets[1](x)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, ref)) and all(torch.equal(a, b[:1]) for a, b in zip(first, ref))
+
+
+def test_a_layer_made_inside_a_capture():
+    n, k = 64, 200
+    g = torch.Generator().manual_seed(2)
+    x, w = torch.randn(50, k, generator=g).cuda(), torch.randn(n, k, generator=g).cuda()
+    Int8Linear(w)(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = Int8Linear(w)(x)
+    for seed in range(3):
+        w.copy_(torch.randn(n, k, generator=g))
+        ref = Int8Linear(w)(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref)

@@ -12,6 +12,8 @@ output channel (y3_linear_i8, include/yolo3hip.h):
 The sum is exact, so a row's result does not depend on the rows beside it.  A row with a NaN or an infinity gives NaN.
 `Network(..., int8=True)` runs its 1x1 convolutions this way.  Calls are asynchronous on the current stream of the
 layer's device; nothing is kept from one call for the next, so calls on several streams and in HIP graphs are independent.
+A layer waits for its weights to be laid out before it is returned, so any stream may call it; one that is made inside a
+capture holds them after the first replay.
 There is no gradient (the package is inference only).
 """
 import collections
@@ -122,6 +124,10 @@ class Int8Linear(object):
         with torch.cuda.device(self.device):
             _lib.check(lib.y3_linear_i8_pack(ctypes.byref(d), _CODES[weight.dtype], weight.data_ptr(), self.k,
                                              self._packed.data_ptr(), self.scale.data_ptr(), _stream_of(self.device.index)))
+            # Later calls may be on any stream, and their callers may not know of this launch (a network packs while it
+            # builds a plan): wait for it here, once.  In a capture the graph orders it before the calls that it holds.
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
         self._descs = {}
         self._weights = (self._packed.data_ptr(), self.scale.data_ptr(), self.bias.data_ptr() if self.bias is not None else None)
 
