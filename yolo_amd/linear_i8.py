@@ -18,6 +18,7 @@ There is no gradient (the package is inference only).
 """
 import collections
 import ctypes
+import operator
 
 import torch
 
@@ -86,58 +87,62 @@ def quantize_rows(x):
 
 class Int8Linear(object):
     """weight [n, k]: float32 / bfloat16 (each row quantised here), or int8 with its scale float32 [n].  bias [n] or None.
-    out_dtype torch.bfloat16 (default) or torch.float32; leaky: leaky-ReLU (alpha 0.1) behind the bias."""
+    out_dtype torch.bfloat16 (default) or torch.float32; leaky: leaky-ReLU (alpha 0.1) behind the bias.
+    The attributes are read-only: descriptors and pointers that calls use are kept from the first one on."""
+
+    n, k, device, leaky, out_dtype, bias, scale = (
+        property(operator.attrgetter("_" + name)) for name in ("n", "k", "device", "leaky", "out_dtype", "bias", "scale"))
 
     def __init__(self, weight, bias=None, scale=None, leaky=False, out_dtype=torch.bfloat16, device=None):
         weight = torch.as_tensor(weight)
         if device is None:
             device = weight.device if weight.is_cuda else torch.device("cuda", torch.cuda.current_device())
-        self.device = torch.device(device)
-        if self.device.type != "cuda":
-            raise ValueError("Int8Linear needs a GPU, got device %s" % self.device)
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
+        self._device = torch.device(device)
+        if self._device.type != "cuda":
+            raise ValueError("Int8Linear needs a GPU, got device %s" % self._device)
+        if self._device.index is None:
+            self._device = torch.device("cuda", torch.cuda.current_device())
         if weight.dim() != 2 or weight.dtype not in _CODES:
             raise ValueError("weight must be [n, k] float32, bfloat16 or int8, got %s %r" % (weight.dtype, tuple(weight.shape)))
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("out_dtype must be torch.bfloat16 or torch.float32, got %s" % out_dtype)
         if (weight.dtype == torch.int8) != (scale is not None):
             raise ValueError("scale goes with an int8 weight, and only with one")
-        self.n, self.k = int(weight.shape[0]), int(weight.shape[1])
-        self.leaky, self.out_dtype = bool(leaky), out_dtype
+        self._n, self._k = int(weight.shape[0]), int(weight.shape[1])
+        self._leaky, self._out_dtype = bool(leaky), out_dtype
         lib = _lib.load()
         d = _lib.LinearI8Desc()
-        d.k, d.n = self.k, self.n
+        d.k, d.n = self._k, self._n
         _lib.check(lib.y3_linear_i8_layout(ctypes.byref(d)))
         self._k_pad, self._n_pad = d.k_pad, d.n_pad
-        weight = weight.detach().to(self.device).contiguous()
+        weight = weight.detach().to(self._device).contiguous()
 
         def vector(v, what):
-            v = torch.as_tensor(v).detach().to(device=self.device, dtype=torch.float32).contiguous()
-            if v.shape != (self.n,):
-                raise ValueError("%s must have shape (%d,), got %r" % (what, self.n, tuple(v.shape)))
+            v = torch.as_tensor(v).detach().to(device=self._device, dtype=torch.float32).contiguous()
+            if v.shape != (self._n,):
+                raise ValueError("%s must have shape (%d,), got %r" % (what, self._n, tuple(v.shape)))
             return v
 
-        self.bias = vector(bias, "bias") if bias is not None else None
-        self.scale = vector(scale, "scale") if scale is not None else torch.empty(self.n, dtype=torch.float32, device=self.device)
-        self._packed = torch.empty(self._k_pad * self._n_pad, dtype=torch.int8, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(lib.y3_linear_i8_pack(ctypes.byref(d), _CODES[weight.dtype], weight.data_ptr(), self.k,
-                                             self._packed.data_ptr(), self.scale.data_ptr(), _stream_of(self.device.index)))
+        self._bias = vector(bias, "bias") if bias is not None else None
+        self._scale = vector(scale, "scale") if scale is not None else torch.empty(self._n, dtype=torch.float32, device=self._device)
+        self._packed = torch.empty(self._k_pad * self._n_pad, dtype=torch.int8, device=self._device)
+        with torch.cuda.device(self._device):
+            _lib.check(lib.y3_linear_i8_pack(ctypes.byref(d), _CODES[weight.dtype], weight.data_ptr(), self._k,
+                                             self._packed.data_ptr(), self._scale.data_ptr(), _stream_of(self._device.index)))
             # Later calls may be on any stream, and their callers may not know of this launch (a network packs while it
             # builds a plan): wait for it here, once.  In a capture the graph orders it before the calls that it holds.
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream().synchronize()
         self._descs = {}
-        self._weights = (self._packed.data_ptr(), self.scale.data_ptr(), self.bias.data_ptr() if self.bias is not None else None)
+        self._weights = (self._packed.data_ptr(), self._scale.data_ptr(), self._bias.data_ptr() if self._bias is not None else None)
 
     def _desc(self, key):
         """(descriptor, workspace bytes) of a call's shape."""
         code, rows, x_ld, out_ld = key
         d = _lib.LinearI8Desc()
-        d.dtype, d.out_dtype, d.k, d.n, d.rows = code, _CODES[self.out_dtype], self.k, self.n, rows
+        d.dtype, d.out_dtype, d.k, d.n, d.rows = code, _CODES[self._out_dtype], self._k, self._n, rows
         d.x_ld, d.out_ld, d.k_pad, d.n_pad = x_ld, out_ld, self._k_pad, self._n_pad
-        d.flags = _lib.CONV_LEAKY if self.leaky else 0
+        d.flags = _lib.CONV_LEAKY if self._leaky else 0
         need = ctypes.c_int64(0)
         _lib.check(_lib.load().y3_linear_i8_workspace_bytes(ctypes.byref(d), ctypes.byref(need)))
         if len(self._descs) >= 256:         # shapes of a service come and go
@@ -148,7 +153,7 @@ class Int8Linear(object):
     def __call__(self, x, scale=None, out=None):
         """x [..., k] float32 / bfloat16, or int8 with scale float32 [...].  Returns [..., n] (in `out` if given)."""
         _check_input(x, "x")
-        device = self.device
+        device = self._device
         if x.device != device:
             raise ValueError("x is on %s, the layer on %s" % (x.device, device))
         if device.index != torch.cuda.current_device():         # launches go to the current device
@@ -159,18 +164,18 @@ class Int8Linear(object):
             raise ValueError("x must be float32, bfloat16 or int8, got %s" % x.dtype)
         if (code == _lib.Y3_I8) != (scale is not None):
             raise ValueError("scale goes with int8 rows, and only with them")
-        m = _rows_of(x, self.k, "x")
+        m = _rows_of(x, self._k, "x")
         rows = m.shape[0]
-        shape = (rows, self.n) if m is x else x.shape[:-1] + (self.n,)
+        shape = (rows, self._n) if m is x else x.shape[:-1] + (self._n,)
         if out is None:
-            out = x.new_empty(shape, dtype=self.out_dtype)
-            out_ld = self.n
+            out = x.new_empty(shape, dtype=self._out_dtype)
+            out_ld = self._n
         else:
-            if out.dtype != self.out_dtype or out.shape != shape or out.device != device:
-                raise ValueError("out must be %s %r on %s" % (self.out_dtype, tuple(shape), device))
-            flat = out.view(-1, self.n) if rows else out            # (a view: rows at one stride, or this raises)
-            out_ld = flat.stride(0) if rows > 1 else self.n
-            if (self.n > 1 and rows and flat.stride(1) != 1) or out_ld < self.n:
+            if out.dtype != self._out_dtype or out.shape != shape or out.device != device:
+                raise ValueError("out must be %s %r on %s" % (self._out_dtype, tuple(shape), device))
+            flat = out.view(-1, self._n) if rows else out            # (a view: rows at one stride, or this raises)
+            out_ld = flat.stride(0) if rows > 1 else self._n
+            if (self._n > 1 and rows and flat.stride(1) != 1) or out_ld < self._n:
                 raise ValueError("out must have adjacent elements in each row and rows that do not overlap")
         if rows == 0:
             return out
@@ -180,9 +185,9 @@ class Int8Linear(object):
                 raise ValueError("scale must be float32 %r on %s" % (tuple(x.shape[:-1]), device))
             scale = scale.contiguous()
             scale_ptr = scale.data_ptr()
-            m, x_ld = _eight_bit_rows(m, self.n)
+            m, x_ld = _eight_bit_rows(m, self._n)
         else:
-            x_ld = m.stride(0) if rows > 1 else self.k
+            x_ld = m.stride(0) if rows > 1 else self._k
         key = (code, rows, x_ld, out_ld)
         dref, need = self._descs.get(key) or self._desc(key)
         ws = x.new_empty(need, dtype=torch.uint8) if need else None
