@@ -80,3 +80,19 @@ def test_a_layer_made_inside_a_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, ref)
+
+
+def test_a_layer_keeps_its_own_scale_and_bias():
+    n, k = 40, 100
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(7, k, generator=g).cuda()
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8).cuda()
+    scale, bias = torch.rand(n, generator=g).cuda(), torch.randn(n, generator=g).cuda()
+    lay = Int8Linear(w, scale=scale, bias=bias)
+    ref = lay(x)
+    for t in (w, scale, bias):
+        t.zero_()
+    assert torch.equal(lay(x), ref)
+    wide = torch.randn(n, 2, generator=g).double()           # other types and strides are copied as they were
+    a, b = Int8Linear(w, scale=wide[:, 0], bias=wide[:, 1]), Int8Linear(w, scale=wide[:, 0].float().cuda(), bias=wide[:, 1].float().cuda())
+    assert torch.equal(a(x), b(x))

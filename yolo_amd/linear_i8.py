@@ -118,10 +118,11 @@ class Int8Linear(object):
         weight = weight.detach().to(self._device).contiguous()
 
         def vector(v, what):
-            v = torch.as_tensor(v).detach().to(device=self._device, dtype=torch.float32).contiguous()
+            v = torch.as_tensor(v).detach()
             if v.shape != (self._n,):
                 raise ValueError("%s must have shape (%d,), got %r" % (what, self._n, tuple(v.shape)))
-            return v
+            # (a copy: the caller's tensor may change or be freed, like the weight it was given with)
+            return torch.empty(self._n, dtype=torch.float32, device=self._device).copy_(v)
 
         self._bias = vector(bias, "bias") if bias is not None else None
         self._scale = vector(scale, "scale") if scale is not None else torch.empty(self._n, dtype=torch.float32, device=self._device)
