@@ -337,9 +337,10 @@ __global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void 
         big = vmax_raw(big, vmax[g]);
     }
     // exp(x - M) as exp2(x log2 e - fl(M log2 e)), one fused operation: the rounding r of M log2 e is in every exponent
-    // alike and comes out of the sums behind the loop.  That does not hold for magnitudes whose product overflows, and
-    // 0 * -inf makes S a NaN where there are impossible classes: such waves, and those with lanes that got nothing or only
-    // logits below -1e37, do it the long way.
+    // alike and comes out of the sums behind the loop.  |r| <= 64 keeps every sum (32 terms of at most 2^64 * 64) and the
+    // factor 2^-r normal numbers; from |M| = 7e8 on r can be larger.  Magnitudes whose product overflows have no such form,
+    // and 0 * -inf makes S a NaN where there are impossible classes: such waves, and those with lanes that got nothing or
+    // only logits below -1e37, do it the long way.
     Sums s = {big, 0.0f, 0.0f};
     const float ml = big * LOG2E;
     unseen();
@@ -351,14 +352,14 @@ __global__ __launch_bounds__(STEP) __attribute__((amdgpu_waves_per_eu(8))) void 
             s.z += e;
             s.s = fmaf(e, y, s.s);
         }
+    const float off = fmaf(big, LOG2E, -ml);                     // r
     {
-        const float r = fmaf(big, LOG2E, -ml);
-        s.s = fmaf(-r, s.z, s.s) * LN2;
-        const float f = __builtin_amdgcn_exp2f(-r);
+        s.s = fmaf(-off, s.z, s.s) * LN2;
+        const float f = __builtin_amdgcn_exp2f(-off);
         s.z *= f;
         s.s *= f;
     }
-    if (__ballot(!(fabsf(big) < 1e37f) || s.s != s.s)) {
+    if (__ballot(!(fabsf(big) < 1e37f) || !(fabsf(off) <= 64.0f) || s.s != s.s)) {
         const auto real = [&](int g, int j) {
             const int c = first_of(g) + j;
             return c >= c0 && c < c1 && tid + g * STEP < vecs ? value(g, j) : ninf;
