@@ -2,11 +2,13 @@
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from oracle import darknet as od
 from yolo_amd import build_model, config
 from yolo_amd import darknet_weights as dw
-from yolo_amd.linear_i8 import Int8Linear
+from yolo_amd.class_probs import log_probs
+from yolo_amd.linear_i8 import Int8Linear, quantize_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +98,25 @@ def test_a_layer_keeps_its_own_scale_and_bias():
     wide = torch.randn(n, 2, generator=g).double()           # other types and strides are copied as they were
     a, b = Int8Linear(w, scale=wide[:, 0], bias=wide[:, 1]), Int8Linear(w, scale=wide[:, 0].float().cuda(), bias=wide[:, 1].float().cuda())
     assert torch.equal(a(x), b(x))
+
+
+def test_gradients_of_a_call_are_refused():
+    """Of every tensor that a call takes, in both directions of differentiation; without gradients they all pass."""
+    lay = Int8Linear(torch.ones(8, 32), out_dtype=torch.float32)
+    x, q, s, y = torch.ones(4, 32).cuda(), torch.ones(4, 32, dtype=torch.int8).cuda(), torch.ones(4).cuda(), torch.empty(4, 8).cuda()
+    lq = Int8Linear(torch.ones(8, 32, dtype=torch.int8), scale=torch.ones(8), out_dtype=torch.float32)
+    ids = torch.zeros(4, dtype=torch.int64).cuda()
+    calls = [(x, lambda t: lay(t)), (x, lambda t: quantize_rows(t)), (s, lambda t: lq(q, scale=t)), (y, lambda t: lay(x, out=t)),
+             (x, lambda t: log_probs(t, ids, top=2)), (s, lambda t: log_probs(x, ids, out=(t, torch.empty(4, device="cuda"), None, None))),
+             (s, lambda t: log_probs(x, ids, out=(torch.empty(4, device="cuda"), t, None, None)))]
+    for t, call in calls:
+        call(t)
+        track = t.clone().requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            call(track)
+        with torch.no_grad():
+            call(track)
+        with forward_ad.dual_level():
+            call(t)
+            with pytest.raises(ValueError, match="tangent"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))

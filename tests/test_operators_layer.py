@@ -1,5 +1,7 @@
 """What may be done to a layer of the 8-bit product after it was made (no GPU)."""
 import pytest
+import torch
+from torch.autograd import forward_ad
 
 from yolo_amd.linear_i8 import Int8Linear
 
@@ -13,3 +15,19 @@ def test_attributes_are_read_only(name):
     with pytest.raises(AttributeError):
         setattr(lay, name, "other")
     assert getattr(lay, name) == "value"
+
+
+@pytest.mark.parametrize("which", ["weight", "bias", "scale"])
+def test_gradients_of_a_layer_are_refused(which):
+    def make(track):
+        t = {"weight": torch.ones(8, 32), "bias": torch.ones(8), "scale": None}
+        if which == "scale":
+            t["weight"], t["scale"] = torch.ones(8, 32, dtype=torch.int8), torch.ones(8)
+        t[which] = track(t[which])
+        return Int8Linear(t["weight"], bias=t["bias"], scale=t["scale"], device="cuda:0")
+
+    with pytest.raises(ValueError, match="gradient"):
+        make(lambda v: v.requires_grad_())
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="tangent"):
+            make(lambda v: forward_ad.make_dual(v, torch.ones_like(v)))

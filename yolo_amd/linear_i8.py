@@ -14,13 +14,14 @@ The sum is exact, so a row's result does not depend on the rows beside it.  A ro
 layer's device; nothing is kept from one call for the next, so calls on several streams and in HIP graphs are independent.
 A layer waits for its weights to be laid out before it is returned, so any stream may call it; one that is made inside a
 capture holds them after the first replay.
-There is no gradient (the package is inference only).
+There is no gradient (the package is inference only): tensors that require one, or carry a tangent, are refused.
 """
 import collections
 import ctypes
 import operator
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -42,11 +43,18 @@ def _rows_of(x, k, name):
     return x
 
 
+def _refuse_gradient(t, name, what):
+    """Neither direction of differentiation goes through the kernels: nothing is dropped without a word."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient: %s has none (use torch.no_grad())" % (name, what))
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError("%s carries a tangent: %s has no forward derivative" % (name, what))
+
+
 def _check_input(x, name):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("%s must be a tensor on the GPU" % name)
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("%s requires a gradient: the 8-bit product has none (use torch.no_grad())" % name)
+    _refuse_gradient(x, name, "the 8-bit product")
 
 
 def _eight_bit_rows(x, n):
@@ -108,6 +116,9 @@ class Int8Linear(object):
             raise ValueError("out_dtype must be torch.bfloat16 or torch.float32, got %s" % out_dtype)
         if (weight.dtype == torch.int8) != (scale is not None):
             raise ValueError("scale goes with an int8 weight, and only with one")
+        for t, name in ((weight, "weight"), (bias, "bias"), (scale, "scale")):
+            if isinstance(t, torch.Tensor):
+                _refuse_gradient(t, name, "the 8-bit product")
         self._n, self._k = int(weight.shape[0]), int(weight.shape[1])
         self._leaky, self._out_dtype = bool(leaky), out_dtype
         lib = _lib.load()
@@ -172,6 +183,7 @@ class Int8Linear(object):
             out = x.new_empty(shape, dtype=self._out_dtype)
             out_ld = self._n
         else:
+            _refuse_gradient(out, "out", "the 8-bit product")
             if out.dtype != self._out_dtype or out.shape != shape or out.device != device:
                 raise ValueError("out must be %s %r on %s" % (self._out_dtype, tuple(shape), device))
             flat = out.view(-1, self._n) if rows else out            # (a view: rows at one stride, or this raises)
@@ -184,6 +196,7 @@ class Int8Linear(object):
         if code == _lib.Y3_I8:
             if scale.dtype != torch.float32 or scale.device != device or scale.shape not in (x.shape[:-1], (rows,)):
                 raise ValueError("scale must be float32 %r on %s" % (tuple(x.shape[:-1]), device))
+            _refuse_gradient(scale, "scale", "the 8-bit product")
             scale = scale.contiguous()
             scale_ptr = scale.data_ptr()
             m, x_ld = _eight_bit_rows(m, self._n)
