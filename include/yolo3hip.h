@@ -314,8 +314,9 @@ int y3_linear_i8_pack(const y3_linear_i8_desc *desc, int w_dtype, const void *w,
 int y3_linear_i8_workspace_bytes(const y3_linear_i8_desc *desc, int64_t *bytes);
 /* x_scale[rows] with Y3_I8 rows, NULL otherwise.  8-bit rows may start anywhere; those on 16 bytes (x and x_ld
  * multiples of 16, x_ld at least k rounded up to 16) are the fastest and are read up to k rounded up to 16, the last one
- * too.  bias[n] may be NULL.  workspace: 16-byte aligned, of this call alone until it has run.  x and
- * out must not overlap (two channel slices of one buffer do not). */
+ * too.  bias[n] may be NULL.  workspace: 16-byte aligned, of this call alone until it has run.  out and
+ * the workspace must overlap neither each other nor anything that is read (rows of two channel slices of one buffer do
+ * not; nor does what lies between two rows). */
 int y3_linear_i8(const y3_linear_i8_desc *desc, const void *x, const float *x_scale, const void *w_packed,
                  const float *w_scale, const float *bias, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 

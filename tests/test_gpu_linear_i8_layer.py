@@ -120,3 +120,21 @@ def test_gradients_of_a_call_are_refused():
             call(t)
             with pytest.raises(ValueError, match="tangent"):
                 call(forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+def test_vectors_between_the_rows_of_an_output():
+    """Scales and bias in the padding of the output's own buffer, the input in another slice of it: nothing overlaps."""
+    rows, k, n = 33, 24, 16
+    g = torch.Generator().manual_seed(5)
+    buf = torch.randn(rows, 64, generator=g).cuda()
+    x, out = buf[:, :k], buf[:, k:k + n]
+    lay = Int8Linear(torch.randn(n, k, generator=g), out_dtype=torch.float32)
+    ref = lay(x.contiguous())
+    before = buf.clone()
+    scale = buf[5, 44:44 + n]                                # between rows 5 and 6 of `out`
+    scale.copy_(lay.scale)
+    lay._weights = (lay._packed.data_ptr(), scale.data_ptr(), None)
+    lay(x, out=out)
+    before[5, 44:44 + n] = lay.scale
+    before[:, k:k + n] = ref
+    assert torch.equal(buf, before)

@@ -1004,6 +1004,14 @@ bool rows_overlap(const void *a, long a_pitch, long a_row, const void *b, long b
     const long apart = ((long)((uintptr_t)b - (uintptr_t)a) % a_pitch + a_pitch) % a_pitch;
     return apart < a_row || apart + b_row > a_pitch;
 }
+// A block of bytes against rows: between two rows it may lie.
+bool block_overlaps_rows(const void *block, long bytes, const void *base, long pitch, long row, long rows) {
+    if (!block || bytes == 0 || !overlap(block, bytes, base, (rows - 1) * pitch + row)) return false;
+    const long at = (long)((uintptr_t)block - (uintptr_t)base);      // (negative: it reaches into the first row)
+    if (at < 0) return true;
+    const long in_row = at % pitch;
+    return in_row < row || (at / pitch + 1 < rows && in_row + bytes > pitch);
+}
 
 }  // namespace
 
@@ -1017,6 +1025,8 @@ extern "C" int y3_quantize_rows_i8(int dtype, const void *x, int64_t rows, int k
     Y3_REQUIRE(x && q && (scale || dtype == Y3_I8), Y3_E_INVALID, "quantize_rows_i8: null pointer");
     Y3_REQUIRE((uintptr_t)x % es_of(dtype) == 0 && aligned16(q) && (uintptr_t)scale % 4 == 0, Y3_E_ALIGN, "quantize_rows_i8: pointer not aligned");
     Y3_REQUIRE(!overlap(x, ((rows - 1) * x_ld + k) * es_of(dtype), q, rows * q_ld), Y3_E_INVALID, "quantize_rows_i8: x and q overlap");
+    Y3_REQUIRE(dtype == Y3_I8 || !(block_overlaps_rows(scale, rows * 4, x, x_ld * es_of(dtype), (long)k * es_of(dtype), rows) ||
+                                   block_overlaps_rows(scale, rows * 4, q, q_ld, round_up(k, 16), rows)), Y3_E_INVALID, "quantize_rows_i8: scale overlaps x or q");
     const hipStream_t st = (hipStream_t)stream;
     const int fill = (int)round_up(k, 16);
     if (dtype == Y3_I8) hipLaunchKernelGGL(repitch_rows_kernel, dim3(rows_grid((rows + 3) / 4)), dim3(256), 0, st, (const char *)x, (long)x_ld, (long)rows, k, (char *)q, (long)q_ld, fill);
@@ -1041,9 +1051,13 @@ extern "C" int y3_linear_i8_pack(const y3_linear_i8_desc *d, int w_dtype, const 
     if (rc) return rc;
     Y3_REQUIRE(l.k_pad == d->k_pad && l.n_pad == d->n_pad, Y3_E_INVALID, "linear_i8_pack: k_pad %d / n_pad %d are not y3_linear_i8_layout's", d->k_pad, d->n_pad);
     Y3_REQUIRE(w_dtype == Y3_F32 || w_dtype == Y3_BF16 || w_dtype == Y3_I8, Y3_E_INVALID, "linear_i8_pack: dtype %d", w_dtype);
-    Y3_REQUIRE(w_ld >= d->k, Y3_E_INVALID, "linear_i8_pack: w_ld %lld < k", (long long)w_ld);
+    Y3_REQUIRE(w_ld >= d->k && w_ld <= (1ll << 44) / d->n, Y3_E_INVALID, "linear_i8_pack: %d channels of k = %d on w_ld %lld", d->n, d->k, (long long)w_ld);
     Y3_REQUIRE(w && packed && (scale || w_dtype == Y3_I8), Y3_E_INVALID, "linear_i8_pack: null pointer");
     Y3_REQUIRE((uintptr_t)w % es_of(w_dtype) == 0 && aligned16(packed) && (uintptr_t)scale % 4 == 0, Y3_E_ALIGN, "linear_i8_pack: pointer not aligned");
+    const long es = es_of(w_dtype), packed_bytes = (long)d->k_pad * d->n_pad;
+    Y3_REQUIRE(!block_overlaps_rows(packed, packed_bytes, w, w_ld * es, d->k * es, d->n) &&
+               (w_dtype == Y3_I8 || !(block_overlaps_rows(scale, d->n * 4l, w, w_ld * es, d->k * es, d->n) || overlap(scale, d->n * 4l, packed, packed_bytes))), Y3_E_INVALID,
+               "linear_i8_pack: packed, scale and w overlap");
     const hipStream_t st = (hipStream_t)stream;
     const int kb = d->k_pad / 64;
     if (w_dtype == Y3_I8) {
@@ -1078,6 +1092,13 @@ extern "C" int y3_linear_i8(const y3_linear_i8_desc *d, const void *x, const flo
     Y3_REQUIRE(!rows_overlap(x, d->x_ld * xs, (long)d->k * xs, out, d->out_ld * os, (long)d->n * os, d->rows),
                Y3_E_INVALID, "linear_i8: x and out overlap");
     Y3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Y3_E_INVALID, "linear_i8: workspace of %lld bytes, needs %lld", (long long)workspace_bytes, (long long)need);
+    const struct { const void *p; long bytes; } read[4] = {{w, (long)d->k_pad * d->n_pad}, {w_scale, d->n * 4l}, {bias, bias ? d->n * 4l : 0}, {x_scale, x_scale ? d->rows * 4 : 0}};
+    for (const auto &r : read) {
+        Y3_REQUIRE(!block_overlaps_rows(r.p, r.bytes, out, d->out_ld * os, (long)d->n * os, d->rows), Y3_E_INVALID, "linear_i8: out overlaps the weights, the scales or the bias");
+        Y3_REQUIRE(need == 0 || r.bytes == 0 || !overlap(r.p, r.bytes, workspace, need), Y3_E_INVALID, "linear_i8: the workspace overlaps the weights, the scales or the bias");
+    }
+    Y3_REQUIRE(need == 0 || !(block_overlaps_rows(workspace, need, x, d->x_ld * xs, (long)d->k * xs, d->rows) || block_overlaps_rows(workspace, need, out, d->out_ld * os, (long)d->n * os, d->rows)),
+               Y3_E_INVALID, "linear_i8: the workspace overlaps x or out");
     const hipStream_t st = (hipStream_t)stream;
     LinArgs a;
     a.x = (const char *)x; a.x_scale = x_scale; a.x_ld = d->x_ld; a.k16 = (int)round_up(d->k, 16);
