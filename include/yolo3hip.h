@@ -343,8 +343,9 @@ typedef struct y3_log_probs_desc {
 /* row_offsets (nullable): element offset of each row instead of the strides above.  A negative offset skips the row: its
  * outputs stay as they are.  A row that would end behind `extent` gets NaN and the class -1.
  * ids (nullable with logp NULL): a negative id means no class, logp 0; an id >= classes gives NaN.
- * logp[rows], entropy[rows] (nullable), top_ids[rows][top] and top_logp[rows][top] (NULL with top = 0): outside the logits,
- * from the first row's start to the last one's end (`extent` with row_offsets). */
+ * logp[rows], entropy[rows] (nullable), top_ids[rows][top] and top_logp[rows][top] (NULL with top = 0).  Outputs and the
+ * workspace overlap neither each other nor the ids, the offsets or the logits, from the first row's start to the last one's
+ * end (`extent` with row_offsets). */
 int y3_log_probs_workspace_bytes(const y3_log_probs_desc *desc, int64_t *bytes);
 int y3_log_probs(const y3_log_probs_desc *desc, const void *logits, const int64_t *row_offsets, const void *ids, float *logp,
                  float *entropy, int32_t *top_ids, float *top_logp, void *workspace, int64_t workspace_bytes, void *stream);

@@ -714,10 +714,17 @@ extern "C" int y3_log_probs(const y3_log_probs_desc *d, const void *logits, cons
         Y3_REQUIRE((last > whole ? last : whole) + d->classes <= (double)d->extent, Y3_E_INVALID, "log_probs: %lld rows reach behind the extent of %lld elements", (long long)d->rows, (long long)d->extent);
         span = (int64_t)(last > whole ? last : whole) + d->classes;
     }
-    const struct { const void *p; int64_t bytes; } outs[4] = {{logp, d->rows * 4}, {entropy, d->rows * 4}, {top_ids, d->rows * d->top * 4}, {top_logp, d->rows * d->top * 4}};
-    for (const auto &o : outs)
-        Y3_REQUIRE(!o.p || !o.bytes || (uintptr_t)o.p + o.bytes <= (uintptr_t)logits || (uintptr_t)logits + span * (d->dtype == Y3_F32 ? 4 : 2) <= (uintptr_t)o.p, Y3_E_INVALID,
-                   "log_probs: an output overlaps the logits");
+    // what is written: the outputs, and with several chunks the workspace (`need`); what is read: the logits, ids and offsets
+    const struct Block { const void *p; int64_t bytes; } written[5] = {{logp, d->rows * 4}, {entropy, d->rows * 4}, {top_ids, d->rows * d->top * 4}, {top_logp, d->rows * d->top * 4}, {workspace, need}};
+    const Block read[3] = {{logits, span * (d->dtype == Y3_F32 ? 4 : 2)}, {ids, d->rows * (d->ids_64 ? 8 : 4)}, {row_offsets, d->rows * 8}};
+    const auto meet = [](const Block &a, const Block &b) {
+        return a.p && b.p && a.bytes && b.bytes && (uintptr_t)a.p < (uintptr_t)b.p + b.bytes && (uintptr_t)b.p < (uintptr_t)a.p + a.bytes;
+    };
+    for (int i = 0; i < 5; ++i) {
+        for (int j = 0; j < 3; ++j)
+            Y3_REQUIRE(!meet(written[i], read[j]), Y3_E_INVALID, "log_probs: %s overlaps the %s", i < 4 ? "an output" : "the workspace", j == 0 ? "logits" : j == 1 ? "ids" : "row offsets");
+        for (int j = 0; j < i; ++j) Y3_REQUIRE(!meet(written[i], written[j]), Y3_E_INVALID, "log_probs: outputs or the workspace overlap each other");
+    }
     ProbsArgs a;
     a.z = (const char *)logits; a.row_offsets = row_offsets; a.ids = ids; a.logp = logp; a.entropy = entropy; a.top_ids = top_ids; a.top_logp = top_logp;
     a.rows = d->rows; a.group_ld = d->group_ld; a.row_ld = d->row_ld; a.extent = d->extent;
@@ -741,6 +748,11 @@ extern "C" int y3_detection_rows(const y3_decode_desc *d, const int32_t *kept_id
         Y3_REQUIRE(d->grid_h[l] >= 1 && d->grid_w[l] >= 1 && d->head_ld[l] >= d->num_anchors * (5 + d->num_classes), Y3_E_INVALID, "detection_rows: scale %d: grid %d x %d, head_ld %d", l,
                    d->grid_h[l], d->grid_w[l], d->head_ld[l]);
     Y3_REQUIRE(((uintptr_t)kept_idx | (uintptr_t)kept_count | (uintptr_t)row_classes) % 4 == 0 && (uintptr_t)row_offsets % 8 == 0, Y3_E_ALIGN, "detection_rows: pointer not aligned");
+    const int64_t pairs = (int64_t)d->batch * d->num_classes, cap = pairs * max_boxes;
+    const auto meet = [](const void *a, int64_t na, const void *b, int64_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; };
+    const int64_t offsets = cap * 8 * d->num_scales;
+    Y3_REQUIRE(!meet(row_offsets, offsets, row_classes, cap * 4) && !meet(row_offsets, offsets, kept_idx, cap * 4) && !meet(row_offsets, offsets, kept_count, pairs * 4) &&
+               !meet(row_classes, cap * 4, kept_idx, cap * 4) && !meet(row_classes, cap * 4, kept_count, pairs * 4), Y3_E_INVALID, "detection_rows: outputs overlap each other or the kept boxes");
     RowsArgs a;
     a.d = *d; a.kept_idx = kept_idx; a.kept_count = kept_count; a.row_offsets = row_offsets; a.row_classes = row_classes; a.max_boxes = max_boxes;
     hipLaunchKernelGGL(detection_rows_kernel, dim3(d->batch), dim3(256), 0, (hipStream_t)stream, a);
