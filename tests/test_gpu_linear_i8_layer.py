@@ -138,3 +138,13 @@ def test_vectors_between_the_rows_of_an_output():
     before[5, 44:44 + n] = lay.scale
     before[:, k:k + n] = ref
     assert torch.equal(buf, before)
+
+
+def test_rows_past_32_bits_are_refused():
+    """5 or 80 values are what 32 bits hold of these lengths."""
+    one = torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda")
+    z, off = torch.zeros(400, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    for bad in (lambda: quantize_rows(one.expand(1, (1 << 32) + 5)), lambda: log_probs(one.expand(1, (1 << 32) + 80)),
+                lambda: log_probs(z, rows=off, classes=(1 << 32) + 80), lambda: log_probs(z, rows=off, classes=(1 << 24) + 1)):
+        with pytest.raises(ValueError):
+            bad()

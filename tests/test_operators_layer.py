@@ -31,3 +31,10 @@ def test_gradients_of_a_layer_are_refused(which):
     with forward_ad.dual_level():
         with pytest.raises(ValueError, match="tangent"):
             make(lambda v: forward_ad.make_dual(v, torch.ones_like(v)))
+
+
+@pytest.mark.parametrize("n,k", [(1, (1 << 32) + 5), ((1 << 32) + 5, 1), (1, 131072), ((1 << 24) + 1, 1)])
+def test_sizes_past_32_bits_are_refused(n, k):
+    """They are not taken for what is left of them in 32 bits."""
+    with pytest.raises(ValueError, match="at most"):
+        Int8Linear(torch.empty(n, k, dtype=torch.int8, device="meta"), scale=torch.empty(n, device="meta"), device="cuda:0")

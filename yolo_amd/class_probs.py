@@ -14,7 +14,7 @@ import torch
 from . import _lib
 from .linear_i8 import _refuse_gradient, _stream_of
 
-MAX_TOP = 32
+MAX_TOP, MAX_CLASSES = 32, 1 << 24      # what the library takes; its own check sees 32 bits of a size only
 ClassProbs = collections.namedtuple("ClassProbs", "logp entropy top_ids top_logp")
 _DESCS = {}
 
@@ -80,6 +80,8 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
         if logits.dim() < 1 or logits.shape[-1] < 1:
             raise ValueError("logits must be [..., C], got %r" % (tuple(logits.shape),))
         C, lead = logits.shape[-1], logits.shape[:-1]
+        if C > MAX_CLASSES:
+            raise ValueError("%d classes, at most %d" % (C, MAX_CLASSES))
         if len(lead) == 1 and (C == 1 or logits.stride(1) == 1):
             n, group, group_ld, row_ld = lead[0], 1, logits.stride(0), 0
         else:
@@ -92,8 +94,8 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
                 n, group = 0, 1
         extent, rows_ptr = 1 << 42, None
     else:
-        if classes is None or int(classes) < 1:
-            raise ValueError("rows needs classes")
+        if classes is None or not 1 <= int(classes) <= MAX_CLASSES:
+            raise ValueError("rows needs classes, 1 .. %d" % MAX_CLASSES)
         if rows.dtype != torch.int64 or rows.dim() != 1 or rows.device != device:
             raise ValueError("rows must be int64 [R] on %s" % device)
         if not logits.is_contiguous():

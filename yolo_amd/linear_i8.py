@@ -27,6 +27,7 @@ from . import _lib
 
 _CODES = {torch.float32: _lib.Y3_F32, torch.bfloat16: _lib.Y3_BF16, torch.int8: _lib.Y3_I8}
 Int8Rows = collections.namedtuple("Int8Rows", "values scale")
+MAX_K, MAX_N = 131071, 1 << 24          # what the library takes; its own check sees 32 bits of a size only
 
 # the current stream's handle, without making a Stream object (1.7 us of a call that takes 6)
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -83,6 +84,8 @@ def quantize_rows(x):
     if x.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("quantize_rows: float32 or bfloat16, got %s" % x.dtype)
     lead, k = x.shape[:-1], x.shape[-1] if x.dim() else 0
+    if k > MAX_K:
+        raise ValueError("quantize_rows: rows of %d, at most %d" % (k, MAX_K))
     m = _rows_of(x, k, "x")
     rows, pitch = m.shape[0], (k + 15) // 16 * 16
     q = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
@@ -120,6 +123,8 @@ class Int8Linear(object):
             if isinstance(t, torch.Tensor):
                 _refuse_gradient(t, name, "the 8-bit product")
         self._n, self._k = int(weight.shape[0]), int(weight.shape[1])
+        if self._n > MAX_N or self._k > MAX_K:
+            raise ValueError("weight is %d x %d, at most %d x %d" % (self._n, self._k, MAX_N, MAX_K))
         self._leaky, self._out_dtype = bool(leaky), out_dtype
         lib = _lib.load()
         d = _lib.LinearI8Desc()
