@@ -33,7 +33,7 @@ def _two_strides(t):
         return 1, 1, 0, 0
     if len(merged) == 1:
         return merged[0][0], 1, merged[0][1], 0
-    if len(merged) == 2:
+    if len(merged) == 2 and merged[0][0] < 1 << 31:        # (a group is a 32-bit number)
         return merged[0][0] * merged[1][0], merged[0][0], merged[1][1], merged[0][1]
     return None
 
