@@ -150,8 +150,19 @@ class Int8Linear(object):
             # builds a plan): wait for it here, once.  In a capture the graph orders it before the calls that it holds.
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream().synchronize()
+        self._bind()
+
+    def _bind(self):
+        """What calls keep: descriptors by shape, and this object's pointers."""
         self._descs = {}
         self._weights = (self._packed.data_ptr(), self._scale.data_ptr(), self._bias.data_ptr() if self._bias is not None else None)
+
+    def __getstate__(self):                 # (copy, pickle: neither of them is the copy's)
+        return {k: v for k, v in self.__dict__.items() if k not in ("_descs", "_weights")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     def _desc(self, key):
         """(descriptor, workspace bytes) of a call's shape."""
