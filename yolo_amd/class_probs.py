@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .linear_i8 import _refuse_gradient, _stream_of
+from .linear_i8 import _forward_ad, _refuse_gradient, _stream_of
 
 MAX_TOP, MAX_CLASSES = 32, 1 << 24      # what the library takes; its own check sees 32 bits of a size only
 ClassProbs = collections.namedtuple("ClassProbs", "logp entropy top_ids top_logp")
@@ -63,7 +63,9 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
     out: (logp, entropy, top_ids, top_logp) to write into, contiguous; None where there is no such output."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a tensor on the GPU")
-    _refuse_gradient(logits, "logits", "log_probs")
+    forward = _forward_ad._current_level >= 0
+    if forward or logits.requires_grad:
+        _refuse_gradient(logits, "logits", "log_probs")
     if logits.dtype == torch.float32:
         code = _lib.Y3_F32
     elif logits.dtype == torch.bfloat16:
@@ -130,7 +132,7 @@ def log_probs(logits, ids=None, top=0, rows=None, classes=None, out=None):
                 raise ValueError("out: logp goes with ids, top_ids and top_logp with top")
             if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous()):
                 raise ValueError("out: expected contiguous %s %r on %s" % (dtype, tuple(shape), device))
-            if t is not None:
+            if t is not None and (forward or t.requires_grad):
                 _refuse_gradient(t, "out", "log_probs")
     if n and (ids is not None or top or entropy is not None):
         dref, need = _descriptor((code, C, n, group, group_ld, row_ld, top, ids_64, extent))

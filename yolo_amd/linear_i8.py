@@ -45,7 +45,8 @@ def _rows_of(x, k, name):
 
 
 def _refuse_gradient(t, name, what):
-    """Neither direction of differentiation goes through the kernels: nothing is dropped without a word."""
+    """Neither direction of differentiation goes through the kernels: nothing is dropped without a word.  (Where every call
+    passes, its callers look at requires_grad and the level themselves first: 0.1 us each.)"""
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires a gradient: %s has none (use torch.no_grad())" % (name, what))
     if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
@@ -55,7 +56,8 @@ def _refuse_gradient(t, name, what):
 def _check_input(x, name):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("%s must be a tensor on the GPU" % name)
-    _refuse_gradient(x, name, "the 8-bit product")
+    if x.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_gradient(x, name, "the 8-bit product")
 
 
 def _eight_bit_rows(x, n):
