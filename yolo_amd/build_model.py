@@ -98,7 +98,7 @@ class _CompiledPlan(object):
     def decode_launchers(self, pp):
         """Launch list of this plan with the YOLO decode fused into the head convolutions (y3_conv2d_head_decode), for
         the thresholds / anchors of PostProcessor `pp`, or None when a head launch does not qualify (small batches,
-        fp32 mode, 2-anchor heads ...): then the caller runs the plain plan and y3_decode.  Returns (desc, launchers)."""
+        fp32 mode, 8-bit heads, 2-anchor heads ...): then the caller runs the plain plan and y3_decode.  Returns (desc, launchers)."""
         key = id(pp)
         hit = self._decode.get(key)
         if hit is None:
@@ -359,7 +359,8 @@ class Network(object):
         # SLOWER per layer inside the network (profiles/r03l), so off unless asked for (YOLO_AMD_BALANCED=1: A/B)
         self.balanced = (os.environ.get("YOLO_AMD_BALANCED", "0") == "1") if balanced is None else bool(balanced)
         # 8-bit products (linear_i8.py) for the 1x1 convolutions that are launches of their own, the heads included: pixels
-        # quantised one by one, weights per output channel, sums exact; everything else stays as it is
+        # quantised one by one, weights per output channel, sums exact; everything else stays as it is.  (An 8-bit head has
+        # no decode in its epilogue: decode_launchers.)
         self.int8 = bool(int8)
         if self.int8 and self.dtype != "bf16":
             raise ValueError("int8 goes with dtype 'bf16' (what surrounds the 8-bit products)")

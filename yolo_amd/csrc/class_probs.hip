@@ -195,13 +195,13 @@ __global__ __launch_bounds__(256) void probs_lanes_kernel(const ProbsArgs p) {
 // those, the top-th largest of 64 groups' maxima (found by bisection of its upper bits, one ballot each) is a bound that at
 // least `top` logits reach and few others do: those are listed, and ranked by counting the larger keys.  A list that
 // overflows (hundreds of equal logits at the border) is settled by one search per alternative.  A row of up to 2048 (4096)
-// logits is one wave's (two waves'): 20000 rows of 2000 bf16 27 us, by four waves 91.
+// logits is one wave's (two waves'): 20000 rows of 2000 bf16 29 us, by four waves 91.
 // Rows of more than one chunk leave {M, Z, S}, the id's logit and the chunk's first `top` keys in the workspace for
 // probs_join_kernel, which merges them in a fixed order.  One workgroup walking a whole row instead: 31 us for one row of
 // 128000 (its exponentials alone keep one CU busy for 9 us), 98 us for 4096 rows of 32001; chunks of 4096 or 2048 logits:
 // 75 and 87 us for the latter against 72.
-//   Bound by vector issue (70 % busy) and memory: 4096 rows of 32001 bf16, 262 MB, 67 us with the join's 6; vectors from the
-//   row's first 16-byte border on, its ends one by one: 71.  One row of 128000: 7 us and 6, all of it latency.
+//   Bound by vector issue (70 % busy) and memory: 4096 rows of 32001 bf16, 262 MB, 73 us with the join (of 32000 68);
+//   vectors from the row's first 16-byte border on, its ends one by one: 78.  One row of 128000: 7 us and 6, all of it latency.
 constexpr int LIST = 512, CHUNK_THREADS = 256;
 
 typedef unsigned long long u64;

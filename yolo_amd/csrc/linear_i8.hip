@@ -143,7 +143,7 @@ template <int LPR, typename F> __device__ __forceinline__ unsigned lanes_max(uns
 // ---- rows -> 8-bit rows + scales --------------------------------------------------------------------------------
 // TPR threads per row, 256 / TPR rows per workgroup (TPR = 64: a wave each), a thread's NI chunks kept in registers between
 // the maximum and the division; rows of more than 8 TPR NI values are read twice, the second time from cache.  Bound by
-// memory, or by the latency of one round trip: 24 rows of 8192 bf16 3.5 us.
+// memory, or by the latency of one round trip: 24 rows of 8192 bf16 3.4 us, 8192 x 8192 fp32 63 us, 5.3 TB/s.
 template <int DT, int TPR, int NI>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void quant_rows_kernel(const char *x, long x_ld, long rows, int k, char *q, long q_ld, int k_fill, float *scale) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1, WAVES = TPR / 64;
@@ -259,8 +259,9 @@ __global__ __launch_bounds__(256) void pack_float_kernel(const char *w, long ld,
 // from 8-bit rows in slabs of k, the next one requested before this one is multiplied -- and every wave reads its weights as
 // whole fragments straight into registers, one k-block ahead (waves along k: four): weights are used by one wave each, LDS
 // would only add a copy.  Waves along k take aligned 8-bit rows as fragments from memory as well.
-//   Bound by: few rows, the weights' way from memory (1 x 4096 -> 4096, 17 MB: 5.0 us); the middle, the latencies of rows,
-//   weights and stores in turn (1777 x 1003 -> 777 fp32 10 us, 7.4 without the products); many rows, the CUs' reads of
+//   Bound by: few rows, the row's way from memory and its quantisation, then the weights', which are requested behind them
+//   (1 x 4096 -> 4096, 17 MB: 5.0 us); the middle, the latencies of rows, weights and stores in turn (1777 x 1003 -> 777
+//   fp32 10 us, 7.4 without the products); many rows, the CUs' reads of
 //   weights from L2 and the stores, all workgroups in the same phase (23104 x 1024 -> 512: 24 us, 15.8 without the products,
 //   21.3 without the stores).  Four k-blocks of weights ahead, or 96 and 128 rows at two waves a SIMD: no faster.
 //   LDS: rows on a pitch of 32 bytes more than their length (16 rows on 16 different 16-byte slots), then per row its scale,
@@ -431,8 +432,11 @@ __device__ __forceinline__ void store_block(const LinArgs &p, char *base, int fr
 // under its products and stores.  LDS holds two panels, so that one barrier per panel is enough.  The waves of a SIMD
 // belong to different workgroups, so that one's quantisation and stores (vector ALU) run beside the other's products; one
 // workgroup of eight waves and 64 rows, all in step, took 37 us for 92416 x 512 -> 256, the panel kernel 38 us.  Bound by
-// memory: 92416 x 512 -> 256 bf16 34 us, 4.2 TB/s.  Output rows that lie end to end but not on 16 bytes are put together in
-// LDS (92416 x 256 -> 255 fp32 32 us, stored quad by quad 39; bf16 27, 35; rows on 16 bytes: 256 bf16 39 that way, 26).
+// memory: 92416 x 512 -> 256 bf16 34.5 us, 4.1 TB/s.  Output rows that lie end to end but not on 16 bytes are put together
+// in LDS (in a graph over different inputs and outputs: 92416 x 256 -> 255 fp32 34 us, stored quad by quad 40; bf16 28, 34;
+// rows on 16 bytes, 256 channels, are not: bf16 38 that way, 26).  fp32 rows of k > 256 with n > 128 have 12 to 40 registers
+// of the rows on their way in memory (92416 x 512 -> 256 in a graph 66 us, its bytes 46), ragged ones of k 129 to 256 with n
+// <= 128 19.
 constexpr int RS_THREADS = 256, RS_ROWS = 32;
 
 // Workgroups per CU: what the registers allow for up to 128 channels (100000 x 100 -> 64 11.7 us, with two 15.9; 1478656 x 128
@@ -560,7 +564,8 @@ void linear_i8_resident_kernel(const LinArgs p, int panels) {
     }
 }
 
-// (registers: the widest kernels and those with fp32 rows in flight take two workgroups per CU, the others three)
+// (registers: the widest kernels, 8-bit rows and fp32 rows of up to 32 a workgroup take two workgroups per CU, the others
+// three; 32 registers of 64 fp32 rows' kernel are in memory, 8 and 17 of the 64 x 512 ones of 8-bit rows, 2 of bf16 rows')
 template <int XT, int RT, int NT, int WK>
 __global__ __launch_bounds__(PN_THREADS) __attribute__((amdgpu_waves_per_eu(NT == 4 || XT >= Y3_I8 || (XT == Y3_F32 && RT <= 2) ? 4 : 6)))
 void linear_i8_panel_kernel(const LinArgs p) {

@@ -99,7 +99,7 @@ def predict_batch(output_nodes, anchors, num_classes, input_shape, image_shape):
 def detect_batch(output_nodes, images, anchors, num_classes, input_shape, image_shape, chunk=None, want_heads=False):
     """Images -> detections in one go: what the reference's `sess.run(predict(output_nodes, ...), {input: images})`
     evaluates (inference.py:88-167, 277).  output_nodes: what `yolo()` returned (or a build_model.Network).  The decode
-    of each scale runs inside its head convolution where the plan allows it, so the fp32 heads are not read back (nor
+    of each scale runs inside its head convolution where the plan allows it (not with int8), so the fp32 heads are not read back (nor
     written, unless want_heads); otherwise this is `predict_batch(output_nodes(images), ...)`.  Same results either way.
     Returns postprocess.Detections, or (Detections, heads) with want_heads."""
     net = getattr(output_nodes, "net", output_nodes)

@@ -117,7 +117,7 @@ class PostProcessor(object):
 
     def detect(self, net, images, image_shapes, chunk=None, want_heads=False, trace=None, trace_filter=None):
         """The whole step on a build_model.Network: backbone -> decode -> NMS -> pack, with the decode of each scale
-        fused into its head convolution's epilogue where the plan allows (bf16, launches on the 256 / 192-pixel tiles:
+        fused into its head convolution's epilogue where the plan allows (bf16 heads, launches on the 256 / 192-pixel tiles:
         the fp32 heads are then never read back, and not even written unless want_heads), else backbone + y3_decode.
         Same records, same detections either way (tests/test_gpu_e2e.py).  Returns (Detections, heads or None)."""
         images = images if isinstance(images, torch.Tensor) else torch.as_tensor(np.asarray(images), dtype=torch.float32)
