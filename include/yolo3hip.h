@@ -2,7 +2,7 @@
  * YOLOv3 inference hot path of viplix3/YOLO.
  *
  * The reference has no FFI layer of its own (it is pure Python over TensorFlow
- * 1.12 ops, SURVEY.md 8b); each entry point below replaces the TF op call
+ * 1.12 ops); each entry point below replaces the TF op call
  * site(s) cited beside it.  Conventions:
  *   - plain pointers and ints only; every pointer is a DEVICE pointer unless it
  *     is a descriptor struct (host) or says "host";
@@ -72,7 +72,7 @@ typedef struct y3_conv_desc {
 } y3_conv_desc;
 
 /* Packed weights: w[n][k], n < n_pad, k < k_pad, k = (kh*ksize + kw)*in_c + c, zero filled
- * beyond out_c / ksize^2*in_c; bias[n_pad] fp32.  The host folds BN (SURVEY 2.3 K3).
+ * beyond out_c / ksize^2*in_c; bias[n_pad] fp32.  The host folds BN.
  * Given in_c/out_c/ksize/dtype this fills k_pad, n_pad and returns which kernel family
  * will run (0 = MFMA implicit GEMM, 1 = direct).  Host-only, no GPU needed. */
 int y3_conv_weight_layout(y3_conv_desc *desc);

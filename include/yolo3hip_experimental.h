@@ -29,7 +29,7 @@ int y3_set_conv_cus(int cus);
 int y3_decode_variant(int v);
 
 /* The all-pairs IoU bitmask form of per-class NMS (BASELINE north_star's sketch), kept for the A/B against the greedy
- * kernels of y3_nms_bucketed (tools/nms_ab.py, DESIGN.md 3.5): bucket -> bitonic sort of each pair's candidates -> one
+ * kernels of y3_nms_bucketed (tools/nms_ab.py): bucket -> bitonic sort of each pair's candidates -> one
  * 64-bit mask word per (row, 64-candidate column block) -> one wavefront per pair scans with the suppressed set in
  * registers.  Same kept indices as y3_nms_bucketed (tests/test_gpu_nms.py).  workspace: y3_nms_workspace_ints() ints;
  * mask: batch * mask_words_per_image 64-bit words, an image needs sum over classes of n * ceil(n / 64); status[b] = 1

@@ -39,7 +39,7 @@ def unique_config_sections(cfg_file):
 
 def parse_layers(config_path, num_classes, num_anchors_per_scale=3, in_channels=3):
     """Walk the cfg exactly as build_model.py:97-255 does and return one dict per
-    non-[net] section (so list index == Darknet layer number, SURVEY 3.2) plus
+    non-[net] section (so list index == Darknet layer number) plus
     the indices of the tensors feeding each [yolo] section (build_model.py:243-247,
     265-267)."""
     assert config_path.endswith(".cfg"), "%s is not a .cfg file" % config_path   # :51

@@ -2,7 +2,7 @@
 """PCIe-inclusive throughput: uint8 images in pinned host memory -> device (second stream) -> y3_letterbox_u8
 (/255, fp32 NHWC) -> backbone + decode + NMS, double-buffered so that the upload of batch n+1 runs under the
 compute of batch n.  bench.py times the path with inputs resident in HBM (the contract); this is the number
-DESIGN.md quotes beside it."""
+beside it."""
 import argparse
 import json
 import os

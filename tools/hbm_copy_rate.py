@@ -1,5 +1,5 @@
 """What a plain device-to-device copy reaches on this GPU: the practical ceiling the HBM-bound kernels
-(decode, stem, the Cout <= 128 convolutions) are held against in DESIGN.md beside the 8 TB/s nominal figure.
+(decode, stem, the Cout <= 128 convolutions) are held against, beside the 8 TB/s nominal figure.
 
     python tools/hbm_copy_rate.py            # one JSON line: GB/s (read + written bytes) per buffer size
 """

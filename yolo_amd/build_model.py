@@ -356,7 +356,7 @@ class Network(object):
         # added in another order, so results are no longer bit-identical across batch sizes / chunking.
         self.splitk = bool(splitk)
         # y3_conv2d_fused_ws for the launches that leave a partial round of 256 x 256 tiles: same bits, but measured 16 - 20 %
-        # SLOWER per layer inside the network (profiles/r03l, DESIGN.md 3.14), so off unless asked for (YOLO_AMD_BALANCED=1: A/B)
+        # SLOWER per layer inside the network (profiles/r03l), so off unless asked for (YOLO_AMD_BALANCED=1: A/B)
         self.balanced = (os.environ.get("YOLO_AMD_BALANCED", "0") == "1") if balanced is None else bool(balanced)
         # 8-bit products (linear_i8.py) for the 1x1 convolutions that are launches of their own, the heads included: pixels
         # quantised one by one, weights per output channel, sums exact; everything else stays as it is.  (An 8-bit head has

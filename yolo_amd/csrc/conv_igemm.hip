@@ -22,8 +22,8 @@
 //
 // What runs by default (conv_variant picks per layer; everything else below is a measured alternative that no
 // layer selects, reachable only in the -DY3_EXPERIMENTS flavour of the library (libyolo3hip_exp.so,
-// include/yolo3hip_experimental.h: y3_set_conv_tile) for A/B runs and the tile-equality tests -- results in
-// DESIGN.md section 3.1.  The default library has no knob, no process-global state and none of the timing paths):
+// include/yolo3hip_experimental.h: y3_set_conv_tile) for A/B runs and the tile-equality tests.  The default
+// library has no knob, no process-global state and none of the timing paths):
 //   256  conv_igemm_kernel<256,256, 8 waves>   Cout >= 256, few rounds         persistent, register epilogue
 //   192  conv_igemm_kernel<192,256, 8 waves>   same, when it saves a round     persistent, register epilogue
 //   257  conv_igemm_ring_kernel<256,128,RING 3> 65..128 output channels (bf16)  two workgroups per CU
@@ -33,7 +33,7 @@
 // Alternatives: 129 (128x256), 258 (256x128, 8 waves), 130/131 (128x128 ring), debug bit 4 (ring for 256/128).
 // Debug bits (high half of y3_set_conv_tile, Y3_EXPERIMENTS only): 1/8/16/32 timing experiments that skip loads or
 // the epilogue (results are garbage), 2 no interleave, 64 force the LDS epilogue, 128 one workgroup per tile.
-// Measured and removed (DESIGN.md section 3.1): cross-tile prefetch, non-temporal epilogue stores / residual loads.
+// Measured and removed: cross-tile prefetch, non-temporal epilogue stores / residual loads.
 #include "common.h"
 #include "conv_common.h"
 #include "decode_box.h"

@@ -614,7 +614,7 @@ extern "C" int y3_nms_bucketed_static(const float *records, const int32_t *cand_
 }
 
 #ifdef Y3_EXPERIMENTS
-// ---- libyolo3hip_exp.so only: the all-pairs IoU bitmask form of per-class NMS, for the A/B in DESIGN.md 3.5 -------
+// ---- libyolo3hip_exp.so only: the all-pairs IoU bitmask form of per-class NMS, for the A/B (tools/nms_ab.py) -------
 // BASELINE's north_star sketches NMS as "a wavefront-level IoU bitmask kernel with an LDS-resident suppression scan".
 // This is that algorithm, written to be fast, so that the choice of the greedy-round kernels above rests on a
 // measurement (tools/nms_ab.py) and not only on the operation count:

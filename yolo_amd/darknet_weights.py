@@ -7,7 +7,7 @@ bias[O]; then the kernel as (O, I, kh, kw).
 
 The writer and the initialiser exist because no pretrained weights are reachable
 offline (the reference fetches them with wget, build_model.py:283-285): benchmarks and
-parity tests run on seeded random weights written in this format (SURVEY 8c).
+parity tests run on seeded random weights written in this format.
 """
 import os
 
@@ -71,7 +71,7 @@ def write_weights(path, layers, params, seen=0):
 
 
 def random_params(layers, seed=0, residual_gain=0.2, weight_gain=1.7, head_gain=0.3):
-    """Seeded init that keeps activations O(1) through 75 layers (SURVEY 8c):
+    """Seeded init that keeps activations O(1) through 75 layers:
     W ~ N(0, weight_gain/(k^2 Cin)), gamma ~ U(.8,1.2), beta ~ N(0,.1), mean ~ N(0,.1),
     var ~ U(.5,1.5), head bias ~ N(0,1).  The gamma of a conv that feeds a [shortcut] is
     scaled by residual_gain (otherwise the 23 residual adds of Darknet-53 double the

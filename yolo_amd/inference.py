@@ -91,7 +91,7 @@ def _postprocessor(anchors, num_classes, input_shape, with_rank=False):
 
 
 def predict_batch(output_nodes, anchors, num_classes, input_shape, image_shape):
-    """Batch form: B independent batch-1 reference runs (SURVEY 8a batch note).
+    """Batch form: B independent batch-1 reference runs.
     image_shape: (h, w) or [B,2].  Returns postprocess.Detections (padded, on the GPU)."""
     return _postprocessor(anchors, num_classes, input_shape)(list(output_nodes), image_shape)
 
@@ -211,7 +211,7 @@ def run_inference(img_path, output_dir, args):
     """inference.py:170-331: every image of img_path -> output_dir/labels/<stem>.txt and the annotated image
     under output_dir/images, FPS excluding the first step.  The reference runs one image per step
     (inference.py:243); `args.batch` = N runs the directory in chunks of N images per step (the last chunk may be
-    shorter).  A batch is B independent batch-1 runs (SURVEY 8a) and the batched plan gives an image the same bits
+    shorter).  A batch is B independent batch-1 runs and the batched plan gives an image the same bits
     whatever the batch size, so the files do not depend on N (tests: byte-identical to batch 1 run with --no_splitk;
     batch 1 splits small launches over k by default, which adds the partial sums in another order)."""
     n_alt = int(getattr(args, "alternatives", 0) or 0)

@@ -186,7 +186,7 @@ def find_stem(layers, inputs, uses, head_of, in_c=3):
 
 RESBLOCK_TILE_W, RESBLOCK_TILE_H = 19, 13      # csrc/conv_resblock.hip: RB_TW, RB_TH
 RESBLOCK_MIN_TILES = 1024                      # fuse only where the launch fills the chip several times over
-# Block widths the automatic mode fuses.  Measured at batch 64 / 608 (DESIGN.md 3.7): C = 128 @152 0.42 ms fused against
+# Block widths the automatic mode fuses.  Measured at batch 64 / 608: C = 128 @152 0.42 ms fused against
 # 0.47 ms in two launches; C = 256 @76 0.317 ms against 0.29 ms (the tile boundary of the fused kernel is bound by the
 # CU's ~15 B/clk memory ingest, which the 1x1 launch, HBM-bound chip-wide, does not pay), so 256 stays un-fused.
 # C = 64 @304 (csrc/conv_resblock64.hip): stem + block 0.764 ms against stem-with-1x1 + 3x3 0.814 ms.

@@ -1,4 +1,4 @@
-"""Batch data-parallel sharding across the GPUs of one node (SURVEY 8e).  The reference is
+"""Batch data-parallel sharding across the GPUs of one node.  The reference is
 single-GPU (config.py:39, inference.py:342-343); images are independent, so rank r simply
 owns the contiguous slice [r*B, (r+1)*B) of the global batch and no collective sits on the
 data path.  The only exchange is one all_gather of per-image detection counts for the node
